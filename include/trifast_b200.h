@@ -342,6 +342,69 @@ int trifast_backward_static_scratch(const trifast_shape* shape,
                                     const trifast_t5* dq, const trifast_t5* dk, const trifast_t5* dv,
                                     const trifast_t4* db, void* stream);
 
+/* ------------------------------------------------------------------ around the attention
+ * The other operators of a pair stack's blocks.  Matrices are row-major; `rows` counts all leading
+ * dimensions together and may be 0.  Pointers are 16-byte aligned, workspaces 256-byte.  Outputs
+ * are dense and overlap no input, except that trifast_dropout_add may write over x or residual.
+ */
+
+/* Layer norm over the last dimension: y = (x - mean) / sqrt(var + eps) * weight + bias. */
+typedef struct trifast_norm {
+  int64_t rows;
+  int64_t ld_x, ld_dy;    /* elements between rows of x and of dy (>= width) */
+  int32_t width;          /* 1 .. 1048576 */
+  int32_t dtype;          /* of x, y and their gradients */
+  int32_t affine_dtype;   /* of weight, bias and their gradients: dtype or TRIFAST_F32 */
+  float eps;
+} trifast_norm;
+
+/* Workspace of the backward when it makes dweight or dbias. */
+size_t trifast_layer_norm_workspace_bytes(const trifast_norm* norm);
+/* weight and bias may be NULL (1 and 0). */
+int trifast_layer_norm(const trifast_norm* norm, const void* x, const void* weight, const void* bias,
+                       void* y, void* stream);
+/* Each of dx, dweight and dbias may be NULL: it is not made. */
+int trifast_layer_norm_backward(const trifast_norm* norm, const void* dy, const void* x,
+                                const void* weight, void* dx, void* dweight, void* dbias,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gated feed-forward block: y = (silu(x w_gate^T) * (x w_up^T)) w_down^T, with w_gate and w_up
+ * (hidden, width) and w_down (width_out, hidden), dense, all of one dtype.  Between the two
+ * products the hidden values are held in that dtype. */
+typedef struct trifast_ff {
+  int64_t rows;
+  int64_t ld_x, ld_dy;    /* elements between rows of x and of dy */
+  int32_t width, hidden, width_out;   /* 1 .. 65536 */
+  int32_t dtype;
+} trifast_ff;
+
+size_t trifast_feed_forward_workspace_bytes(const trifast_ff* ff);
+size_t trifast_feed_forward_backward_workspace_bytes(const trifast_ff* ff);
+int trifast_feed_forward(const trifast_ff* ff, const void* x, const void* w_gate, const void* w_up,
+                         const void* w_down, void* y, void* workspace, size_t workspace_bytes,
+                         void* stream);
+/* dx may be NULL; the three weight gradients are made all or (all NULL) none. */
+int trifast_feed_forward_backward(const trifast_ff* ff, const void* dy, const void* x,
+                                  const void* w_gate, const void* w_up, const void* w_down, void* dx,
+                                  void* dw_gate, void* dw_up, void* dw_down, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Dropout with the residual sum: y = residual + (kept ? x / (1 - p) : 0), on dense (outer, mid, inner)
+ * tensors whose mask has outer x inner entries and is shared along mid.  Entry i is kept if its
+ * word, of 2^32, is not below round(p 2^32); the word is number i % 4 of Philox-4x32-10 at counter
+ * (i / 4, offset) under the key seed + *seed_device (NULL: seed alone; read when the kernel runs, so
+ * that a replayed graph can draw anew).  The gradient with respect to x is the same call on dy
+ * without a residual (NULL). */
+typedef struct trifast_dropout {
+  int64_t outer, mid, inner;
+  int32_t dtype;
+  uint64_t seed, offset;
+  double p;               /* 0 .. 1 */
+} trifast_dropout;
+
+int trifast_dropout_add(const trifast_dropout* dropout, const int64_t* seed_device, const void* x,
+                        const void* residual, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

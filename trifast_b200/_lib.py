@@ -58,6 +58,21 @@ class Plan(C.Structure):
                 ("bwd_fused", C.c_int32), ("bwd_chunks", C.c_int32), ("fwd_kernel", C.c_int32)]
 
 
+class Norm(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("ld_x", C.c_int64), ("ld_dy", C.c_int64), ("width", C.c_int32),
+                ("dtype", C.c_int32), ("affine_dtype", C.c_int32), ("eps", C.c_float)]
+
+
+class FeedForward(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("ld_x", C.c_int64), ("ld_dy", C.c_int64), ("width", C.c_int32),
+                ("hidden", C.c_int32), ("width_out", C.c_int32), ("dtype", C.c_int32)]
+
+
+class Dropout(C.Structure):
+    _fields_ = [("outer", C.c_int64), ("mid", C.c_int64), ("inner", C.c_int64), ("dtype", C.c_int32),
+                ("seed", C.c_uint64), ("offset", C.c_uint64), ("p", C.c_double)]
+
+
 # name -> (restype, argtypes); one entry per declaration in include/trifast_b200.h
 _P = C.POINTER
 SIGNATURES = {
@@ -87,6 +102,15 @@ SIGNATURES = {
     "trifast_host_status_word": (C.c_int, [_P(_P(C.c_uint32))]),
     "trifast_db_push_reduce": (C.c_int, [_P(PushReduce), C.c_void_p]),
     "trifast_db_push_reduce_staging_floats": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "trifast_layer_norm_workspace_bytes": (C.c_size_t, [_P(Norm)]),
+    "trifast_layer_norm": (C.c_int, [_P(Norm)] + [C.c_void_p] * 5),
+    "trifast_layer_norm_backward": (C.c_int, [_P(Norm)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "trifast_feed_forward_workspace_bytes": (C.c_size_t, [_P(FeedForward)]),
+    "trifast_feed_forward_backward_workspace_bytes": (C.c_size_t, [_P(FeedForward)]),
+    "trifast_feed_forward": (C.c_int, [_P(FeedForward)] + [C.c_void_p] * 6 + [C.c_size_t, C.c_void_p]),
+    "trifast_feed_forward_backward": (C.c_int, [_P(FeedForward)] + [C.c_void_p] * 10 +
+                                      [C.c_size_t, C.c_void_p]),
+    "trifast_dropout_add": (C.c_int, [_P(Dropout)] + [C.c_void_p] * 5),
     "trifast_debug_wait_probe": (C.c_int, [C.c_uint32, C.c_void_p]),
     "trifast_backward_static_scratch": (C.c_int, [_P(Shape), _P(T5), _P(T5), _P(T5), _P(T5), _P(T4),
                                                   _P(Mask), _P(T5), C.c_void_p, _P(T5), _P(T5),

@@ -4,7 +4,7 @@
     python -m trifast_b200.build [--force] [--verbose]
 
 Every ``csrc/*.cu`` file is compiled to an object next to it (``csrc/_obj/``) and
-linked into ``trifast_b200/libtrifast_b200.so``; ``csrc/torch_ops.cpp`` is compiled against
+linked into ``trifast_b200/libtrifast_b200.so``; ``csrc/torch_*.cpp`` are compiled against
 the installed PyTorch and linked to it.  Objects are rebuilt when a source or header is newer.  No GPU is needed to build.
 """
 
@@ -22,7 +22,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(CSRC, "_obj")
 LIB = os.path.join(PKG, "libtrifast_b200.so")
-OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
+OPS_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block_ops.cpp")]
 OPS_LIB = os.path.join(PKG, "libtrifast_b200_torch.so")
 
 NVCC_FLAGS = [
@@ -44,8 +44,8 @@ def _newest(paths) -> float:
     return max(os.path.getmtime(p) for p in paths)
 
 
-def _ops_commands(nvcc: str, obj: str):
-    """Compile and link commands of the operator library.
+def _ops_commands(nvcc: str, objs: list):
+    """Compile commands (one per source) and the link command of the operator library.
 
     It links the shared C++ runtime by its file name: a compiler that has only the static one
     (``libstdc++.a``) would put a second copy into the process beside PyTorch's, and the two
@@ -57,12 +57,13 @@ def _ops_commands(nvcc: str, obj: str):
     inc = [f for p in include_paths() + [os.path.join(root, "include")] for f in ("-isystem", p)]
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    compile_cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-Wall",
-                   f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, "-c", OPS_SRC, "-o", obj]
-    link_cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", OPS_LIB, obj, "-L", PKG,
+    compile_cmds = [[os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-Wall",
+                     f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, "-c", src, "-o", obj]
+                    for src, obj in zip(OPS_SRCS, objs)]
+    link_cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", OPS_LIB, *objs, "-L", PKG,
                 "-l:libtrifast_b200.so", "-l:libstdc++.so.6", "-L", libs, "-lc10", "-lc10_cuda",
                 "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libs]
-    return compile_cmd, link_cmd
+    return compile_cmds, link_cmd
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -85,12 +86,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
             jobs.append(cmd)
 
     # the operators, compiled beside the kernels (their link waits for the library)
-    ops_obj = os.path.join(OBJ, "torch_ops.o")
-    ops_compile, ops_link = _ops_commands(nvcc, ops_obj)
-    ops_stale = force or not os.path.exists(ops_obj) or \
-        os.path.getmtime(ops_obj) < max(os.path.getmtime(OPS_SRC), dep_time)
-    if ops_stale:
-        jobs.append(ops_compile)
+    ops_objs = [os.path.join(OBJ, os.path.basename(src)[:-4] + ".o") for src in OPS_SRCS]
+    ops_compiles, ops_link = _ops_commands(nvcc, ops_objs)
+    ops_stale = False
+    for src, obj, cmd in zip(OPS_SRCS, ops_objs, ops_compiles):
+        if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), dep_time):
+            ops_stale = True
+            jobs.append(cmd)
 
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -110,7 +112,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
     if ops_stale or not os.path.exists(OPS_LIB) or \
-            os.path.getmtime(OPS_LIB) < max(os.path.getmtime(ops_obj), os.path.getmtime(LIB)):
+            os.path.getmtime(OPS_LIB) < max(_newest(ops_objs), os.path.getmtime(LIB)):
         _, r = run(ops_link)
         if r.returncode:
             sys.stderr.write(r.stdout + r.stderr)

@@ -354,12 +354,21 @@ int fill_bwd(const trifast_shape* shape, const Common& c, const trifast_t5* d_o,
 // The CUDA error behind the last TRIFAST_ERR_LAUNCH of the calling thread.
 thread_local cudaError_t g_last_cuda_error = cudaSuccess;
 
+}  // namespace
+
 int cuda_rc(cudaError_t e) {
   if (e == cudaSuccess) return TRIFAST_OK;
   g_last_cuda_error = e;
   cudaGetLastError();   // reported here: the next launch's check must not find it again
   return TRIFAST_ERR_LAUNCH;
 }
+
+int device_status(unsigned int** status) {
+  int dev;
+  return device_setup(&dev, status);
+}
+
+namespace {
 
 // The kernels a backward runs on.
 enum BwdKernels { kBwdSimt, kBwdFused, kBwdSplit, kBwdD128 };

@@ -97,6 +97,7 @@ enum DeviceStatusBits : unsigned int {
   kStatusTimeoutBwdFused = 16u,
   kStatusTimeoutProbe = 32u,
   kStatusTimeoutPushReduce = 64u,
+  kStatusTimeoutFeedForward = 128u,
 };
 
 // (out of line, so that the cold path leaves the code of the kernels' loops alone)

@@ -1,0 +1,721 @@
+// The matrix products of the gated feed-forward block
+//     a = X Wg^T,  b = X Wu^T,  h = silu(a) * b,  y = h Wd^T
+// and of its backward pass
+//     dh = dY Wd,  db = dh silu(a),  da = dh b silu'(a),
+//     dX = da Wg + db Wu,  dWg = da^T X,  dWu = db^T X,  dWd = dY^T h
+// on the tensor cores, as one kernel with four epilogues (Mode in ff_gemm.cuh).
+//
+// A tile has 128 rows and up to 256 fp32 columns in TMEM, twice, so that the epilogue of one tile runs
+// under the MMAs of the next.  Operands come in blocks of 64 along the contraction, through a ring of
+// stages that TMA fills (128-byte swizzle).  Both majors are read as they lie: where the contraction
+// runs along a matrix's rows the tile is an MN-major operand of 64-element columns.  CTAs are
+// persistent, one per SM, the tiles of one row block next to one another.
+// Warps 0-7: epilogue (two warpgroups, each half of a tile's columns), 8: TMA, 9: MMA issuer.
+//
+// fp32: every value is the sum of three bf16 ones (ff_support.cu), and a product is the six
+// products of parts that are not below 2^-22 of it, the smallest first.  The accumulators in TMEM round towards
+// zero, so that a long sum drifts (5e-6 of the result over 384 MMAs): a sum ends after 256 of the contraction's
+// largest products, and the epilogue adds the sums up in fp32 registers, rounded to nearest.
+//
+// What bounds it: the tiles' way from L2.  A 128 x 256 tile takes 48 KB per 64 of the contraction, for 512
+// cycles of the tensor pipe.
+
+#include <initializer_list>
+#include <type_traits>
+
+#include "ff_gemm.cuh"
+#include "tc_common.cuh"
+
+namespace trifast {
+namespace ff {
+namespace {
+using namespace tc;
+
+constexpr int kBK = 64;                  // contraction per stage
+constexpr int kTileA = 128 * kBK * 2;    // bytes of an operand tile of 128 rows
+constexpr int kThreads = 320;
+constexpr int kSmemLimit = 232448;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Columns per B matrix (NT), accumulator columns, stages and staging of results by mode.
+template <int MODE, int NT>
+struct Cfg {
+  static constexpr int kAccCols = MODE == kGate ? 2 * NT : MODE == kHidden ? 3 * NT : NT;
+  static constexpr int kBRows = MODE == kGate || MODE == kHidden ? 2 * NT : NT;   // largest of a stage
+  static constexpr int kStageBytes = kTileA + kBRows * kBK * 2;
+  // result tiles of 128 rows x 64 columns
+  static constexpr int kOutTiles = MODE == kGate ? NT / 64 : MODE == kHidden ? 3 : MODE == kLinear ? 2 : 0;
+  static constexpr int kStages = (kSmemLimit - 2048 - kOutTiles * kTileA) / kStageBytes;
+  static constexpr int kBufCols = kAccCols > 128 ? 256 : 128;    // TMEM columns between the two buffers
+  static constexpr int smem_bytes() { return 1024 + 1024 + kStages * kStageBytes + kOutTiles * kTileA; }
+  static_assert(kAccCols <= 256 && kStages >= 4 && smem_bytes() <= kSmemLimit, "tile configuration");
+};
+
+struct Params {
+  CUtensorMap a[3], b[3], out[3];
+  int64_t m[3], n[3], k[3];   // kWeight: of each product; else of product 0 (k: of each phase)
+  int m_tiles[3], n_tiles[3], tiles;
+  int phases;
+  void* y;
+  int64_t ldy;
+  int y_tma;
+  float* partials;
+  int64_t partial_stride;
+  int splits, add;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// A barrier of `threads` threads that tells whether all of them came with `ok`.
+__device__ __forceinline__ bool group_all(int id, int threads, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + e^-a): 0 and 1 at the ends, NaN for NaN
+__device__ __forceinline__ float sigmoid(float a) { return rcp(1.f + ex2(-kLog2e * a)); }
+
+// Pairs of planes (of A, of B) whose products make up a product of fp32 values, the smallest first.
+__device__ __forceinline__ int plane_a(int q) { return (0x001021 >> (4 * q)) & 15; }   // 1 2 0 1 0 0
+__device__ __forceinline__ int plane_b(int q) { return (0x010201 >> (4 * q)) & 15; }   // 1 0 2 0 1 0
+
+// One part of a value and what is left of it: PARTS = 1 rounds to T, PARTS = 3 cuts to bf16, so that three
+// parts hold all 24 bits.
+template <typename T, int PARTS>
+__device__ __forceinline__ uint32_t take_part(float& v0, float& v1) {
+  if constexpr (PARTS == 1) {
+    return pack2<T>(v0, v1);
+  } else {
+    const uint32_t a = __float_as_uint(v0), b = __float_as_uint(v1);
+    v0 -= __uint_as_float(a & 0xffff0000u);
+    v1 -= __uint_as_float(b & 0xffff0000u);
+    return __byte_perm(a, b, 0x7632);
+  }
+}
+
+// Stages of the largest products that one sum in TMEM takes when PARTS is 3 (those of the smaller ones, five
+// times as many, go before the first).
+constexpr int kSumStages = 4;
+__device__ __forceinline__ int sums_of(int blocks) { return blocks <= kSumStages ? 1 : (blocks + kSumStages - 1) / kSumStages; }
+
+struct TileAt {
+  int m0, n0;     // first row and column
+  int job, split;
+};
+
+template <int MODE, int NT>
+__device__ __forceinline__ TileAt tile_at(const Params& p, int t) {
+  TileAt r;
+  r.job = 0;
+  r.split = 0;
+  if constexpr (MODE == kWeight) {
+    r.split = t % p.splits;
+    t /= p.splits;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (r.job == j && t >= p.m_tiles[j] * p.n_tiles[j]) {
+        t -= p.m_tiles[j] * p.n_tiles[j];
+        r.job = j + 1;
+      }
+  }
+  const int nt = p.n_tiles[r.job];
+  r.m0 = (t / nt) * 128;
+  r.n0 = (t % nt) * NT;
+  return r;
+}
+
+// T: type of the operands; PARTS: planes of each (1, or 3 for fp32); OUT: type of kLinear's result.
+template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN>
+__global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<MODE, NT>;
+  constexpr int S = C::kStages;
+  constexpr int FULL = 0, EMPTY = S, ACC_FULL = 2 * S, ACC_EMPTY = 2 * S + 2, NBARS = 2 * S + 4;
+  static_assert(NBARS * 8 <= 240, "barrier area");
+  constexpr int kPairs = PARTS == 1 ? 1 : 6;
+  constexpr bool kAMn = MODE == kWeight;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + 256);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + 260);
+  auto bar = [&](int i) -> uint32_t { return base + 8u * i; };
+  auto a_tile = [&](int s) -> uint32_t { return base + 1024 + s * C::kStageBytes; };
+  auto b_tile = [&](int s) -> uint32_t { return a_tile(s) + kTileA; };
+  constexpr uint32_t out_off = 1024 + S * C::kStageBytes;
+
+  after_previous();
+  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(bar(FULL + s), 1);
+      mbar_init(bar(EMPTY + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), 8);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // blocks of the contraction of phase ph of a tile
+  auto k_range = [&](const TileAt& t, int ph, int& lo, int& hi) {
+    const int blocks = (int)((p.k[MODE == kWeight ? 0 : ph] + kBK - 1) / kBK);
+    lo = 0;
+    hi = blocks;
+    if (MODE == kWeight) {
+      lo = (int)((int64_t)blocks * t.split / p.splits);
+      hi = (int)((int64_t)blocks * (t.split + 1) / p.splits);
+    }
+  };
+  const int phases = MODE == kHidden ? 2 : MODE == kLinear ? p.phases : 1;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA producer
+    int g = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; w < p.tiles && ok; w += gridDim.x) {
+      const TileAt t = tile_at<MODE, NT>(p, w);
+      for (int ph = 0; ph < phases && ok; ++ph) {
+        int lo, hi;
+        k_range(t, ph, lo, hi);
+        const CUtensorMap* ma = &p.a[MODE == kWeight ? t.job : ph];
+        for (int q = 0; q < kPairs && ok; ++q) {
+          const int pa = kPairs == 1 ? 0 : plane_a(q), pb = kPairs == 1 ? 0 : plane_b(q);
+          for (int kb = lo; kb < hi; ++kb, ++g) {
+            const int s = g % S;
+            if (g >= S) ok = mbar_wait(bar(EMPTY + s), ((g / S) - 1) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (elect_one()) {
+              const uint32_t f = bar(FULL + s);
+              const int kc = kb * kBK;
+              if constexpr (MODE == kHidden) {
+                mbar_arrive_expect_tx(f, kTileA + (ph == 0 ? 2 : 1) * NT * kBK * 2);
+                tma_load_3d(a_tile(s), ma, f, kc, t.m0, pa);
+                if (ph == 0) {
+                  tma_load_3d(b_tile(s), &p.b[0], f, kc, t.n0, pb);
+                  tma_load_3d(b_tile(s) + NT * kBK * 2, &p.b[1], f, kc, t.n0, pb);
+                } else {
+                  tma_load_3d(b_tile(s), &p.b[2], f, t.n0, kc, pb);
+                }
+              } else {
+                mbar_arrive_expect_tx(f, C::kStageBytes);
+                if constexpr (kAMn) {
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) tma_load_3d(a_tile(s) + i * 8192, ma, f, t.m0 + 64 * i, kc, pa);
+                } else {
+                  tma_load_3d(a_tile(s), ma, f, kc, t.m0, pa);
+                }
+                if constexpr (MODE == kGate) {
+                  tma_load_3d(b_tile(s), &p.b[0], f, kc, t.n0, pb);
+                  tma_load_3d(b_tile(s) + NT * kBK * 2, &p.b[1], f, kc, t.n0, pb);
+                } else {
+                  const CUtensorMap* mb = &p.b[MODE == kWeight ? t.job : ph];
+                  if constexpr (B_MN) {
+#pragma unroll
+                    for (int i = 0; i < NT / 64; ++i) tma_load_3d(b_tile(s) + i * 8192, mb, f, t.n0 + 64 * i, kc, pb);
+                  } else {
+                    tma_load_3d(b_tile(s), mb, f, kc, t.n0, pb);
+                  }
+                }
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    int g = 0, it = 0;   // running stage, and running sum (a buffer of TMEM)
+    bool ok = true;
+    uint32_t acc = tmem_base;
+    auto open_sum = [&] {
+      acc = tmem_base + (it & 1) * C::kBufCols;
+      if (it >= 2) ok = mbar_wait(bar(ACC_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    };
+    auto close_sum = [&] {
+      if (elect_one()) umma_commit(bar(ACC_FULL + (it & 1)));
+      __syncwarp();
+      ++it;
+    };
+    for (int w = blockIdx.x; w < p.tiles && ok; w += gridDim.x) {
+      const TileAt t = tile_at<MODE, NT>(p, w);
+      open_sum();
+      for (int ph = 0; ph < phases && ok; ++ph) {
+        int lo, hi;
+        k_range(t, ph, lo, hi);
+        const int steps = (hi - lo) * kPairs, small = (hi - lo) * (kPairs - 1);
+        if (PARTS == 3 && ph > 0) {
+          close_sum();
+          open_sum();
+        }
+        // (kLinear's two products add up in one accumulator; kHidden's second phase has its own)
+        bool first = PARTS == 3 || MODE != kLinear || ph == 0;
+        for (int i = 0; i < steps && ok; ++i, ++g) {
+          if (PARTS == 3 && i > small && (i - small) % kSumStages == 0) {
+            close_sum();
+            open_sum();
+            if (!ok) break;
+            first = true;
+          }
+          const int s = g % S;
+          ok = mbar_wait(bar(FULL + s), (g / S) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const bool second = MODE == kHidden && ph == 1;
+            const bool bmn = second || B_MN;
+            const uint32_t idesc = second ? make_idesc(128, NT, kBf16, false, true)
+                                          : make_idesc(128, C::kBRows, kBf16, kAMn, B_MN);
+            const uint32_t d = acc + (second ? 2 * NT : 0);
+            const uint64_t ad = make_smem_desc(a_tile(s), kAMn ? 8192 : 16, 1024, kSwizzle128);
+            const uint64_t bd = make_smem_desc(b_tile(s), bmn ? 8192 : 16, 1024, kSwizzle128);
+            // 16 of the contraction: 32 bytes along a row, or 16 rows of an MN-major tile
+            const uint32_t sa = kAMn ? 2048 >> 4 : 32 >> 4, sb = bmn ? 2048 >> 4 : 32 >> 4;
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk) umma_ss(d, ad + kk * sa, bd + kk * sb, idesc, (kk > 0 || !first) ? 1u : 0u);
+            umma_commit(bar(EMPTY + s));
+          }
+          __syncwarp();
+          first = false;
+        }
+      }
+      if (!ok) break;
+      close_sum();
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int grp = warp >> 2, wq = warp & 3, row = tid & 127;
+    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+    int it = 0;   // running sum
+    bool ok = true;
+    // 16-byte piece `c16` of this thread's row in a 128 x 64 result tile (128-byte swizzle)
+    auto out_piece = [&](int tile, int c16) -> uint4* {
+      return reinterpret_cast<uint4*>(gbase + out_off + tile * kTileA + row * 128 + ((c16 ^ (row & 7)) << 4));
+    };
+    // kHidden's result tiles, and kGate's of 64 columns, are written by both groups
+    constexpr bool kShared = MODE == kHidden || (MODE == kGate && NT == 64);
+    const int bar_id = kShared ? 3 : 1 + grp;
+    constexpr int kBarThreads = kShared ? 256 : 128;
+    const bool leader = kShared ? tid == 0 : row == 0;
+    uint32_t acc = tmem_base;
+    // (all warps of a barrier go on, or none: the barriers below count on it)
+    auto wait_sum = [&] {
+      ok = mbar_wait(bar(ACC_FULL + (it & 1)), (it >> 1) & 1, abort_flag);
+      ok = group_all(bar_id, kBarThreads, ok);
+      tc_fence_after();
+      acc = tmem_base + lane_base + (it & 1) * C::kBufCols;
+    };
+    auto release = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(ACC_EMPTY + (it & 1)));
+      ++it;
+    };
+    // PARTS = 3: this thread's columns of each matrix, added up over the sums
+    constexpr int kCols = NT / 2, kSets = MODE == kGate ? 2 : MODE == kHidden ? 3 : 1;
+    float total[PARTS == 3 ? kSets : 1][PARTS == 3 ? kCols : 1];
+    for (int w = blockIdx.x; w < p.tiles; w += gridDim.x) {
+      const TileAt t = tile_at<MODE, NT>(p, w);
+      bool none = false;   // an empty contraction: its sum is 0, and nothing wrote TMEM
+      if constexpr (MODE == kWeight) {
+        int lo, hi;
+        k_range(t, 0, lo, hi);
+        none = hi <= lo;
+      }
+      if constexpr (PARTS == 1) {
+        wait_sum();
+      } else {
+#pragma unroll
+        for (int m = 0; m < kSets; ++m)
+#pragma unroll
+          for (int e = 0; e < kCols; ++e) total[m][e] = 0.f;
+#pragma unroll
+        for (int ph = 0; ph < 2; ++ph) {
+          if (ph >= phases) continue;
+          int lo, hi;
+          k_range(t, ph, lo, hi);
+          const int sums = sums_of(hi - lo);
+          for (int i = 0; i < sums && ok; ++i) {
+            wait_sum();
+            if (!ok) break;
+            constexpr int kLast = kSets;
+            const int m0 = MODE == kHidden && ph == 1 ? 2 : 0, m1 = MODE == kHidden && ph == 0 ? 2 : kLast;
+#pragma unroll
+            for (int m = 0; m < kSets; ++m) {
+              if (m < m0 || m >= m1) continue;
+#pragma unroll
+              for (int c = 0; c < kCols; c += 32) {
+                float v[32];
+                tmem_ld32(acc + m * NT + grp * kCols + c, reinterpret_cast<uint32_t*>(v));
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) total[m][c + e] += none ? 0.f : v[e];
+              }
+            }
+            release();
+          }
+        }
+      }
+      if (!ok) break;
+      // columns [c, c + 32) of matrix m of this thread's half
+      auto columns = [&](int m, int c, float* v) {
+        if constexpr (PARTS == 3) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = total[m][c + e];
+        } else {
+          tmem_ld32(acc + m * NT + grp * kCols + c, reinterpret_cast<uint32_t*>(v));
+        }
+      };
+      auto loaded = [&](bool last) {
+        if constexpr (PARTS == 1) {
+          tmem_wait_ld();
+          if (last) release();
+        }
+      };
+      if constexpr (MODE == kGate) {
+        float h[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; c += 32) {
+          float a[32], b[32];
+          columns(0, c, a);
+          columns(1, c, b);
+          loaded(c + 32 == kCols);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) h[c + e] = a[e] * sigmoid(a[e]) * b[e];
+        }
+        const int tile = kShared ? 0 : grp, piece = kShared ? grp * (kCols / 8) : 0, col = t.n0 + tile * 64;
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          if (leader) bulk_wait_read();
+          group_sync(bar_id, kBarThreads);
+#pragma unroll
+          for (int c = 0; c < kCols; c += 8) {
+            uint4 u;
+            u.x = take_part<T, PARTS>(h[c], h[c + 1]);
+            u.y = take_part<T, PARTS>(h[c + 2], h[c + 3]);
+            u.z = take_part<T, PARTS>(h[c + 4], h[c + 5]);
+            u.w = take_part<T, PARTS>(h[c + 6], h[c + 7]);
+            *out_piece(tile, piece + (c >> 3)) = u;
+          }
+          fence_async_smem();
+          group_sync(bar_id, kBarThreads);
+          if (leader && col < p.n[0]) {
+            tma_store_3d(&p.out[0], base + out_off + tile * kTileA, col, t.m0, q);
+            bulk_commit();
+          }
+        }
+      } else if constexpr (MODE == kHidden) {
+        static_assert(MODE != kHidden || NT == 64, "result tiles are 64 columns");
+        float r[3][32];
+        {
+          float a[32], b[32], dh[32];
+          columns(0, 0, a);
+          columns(1, 0, b);
+          columns(2, 0, dh);
+          loaded(true);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float s = sigmoid(a[e]), u = a[e] * s;
+            r[0][e] = dh[e] * b[e] * fmaf(u, 1.f - s, s);
+            r[1][e] = dh[e] * u;
+            r[2][e] = u * b[e];
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          if (leader) bulk_wait_read();
+          group_sync(bar_id, kBarThreads);
+#pragma unroll
+          for (int o = 0; o < 3; ++o)
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint4 u;
+              u.x = take_part<T, PARTS>(r[o][c], r[o][c + 1]);
+              u.y = take_part<T, PARTS>(r[o][c + 2], r[o][c + 3]);
+              u.z = take_part<T, PARTS>(r[o][c + 4], r[o][c + 5]);
+              u.w = take_part<T, PARTS>(r[o][c + 6], r[o][c + 7]);
+              *out_piece(o, (grp * 32 + c) >> 3) = u;
+            }
+          fence_async_smem();
+          group_sync(bar_id, kBarThreads);
+          if (leader) {
+#pragma unroll
+            for (int o = 0; o < 3; ++o) tma_store_3d(&p.out[o], base + out_off + o * kTileA, t.n0, t.m0, q);
+            bulk_commit();
+          }
+        }
+      } else if constexpr (MODE == kLinear) {
+        const int64_t gr = (int64_t)t.m0 + row;
+        OUT* yr = reinterpret_cast<OUT*>(p.y) + gr * p.ldy;
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 64) {
+          const int col = t.n0 + grp * kCols + c0;
+          float v[64];
+          columns(0, c0, v);
+          columns(0, c0 + 32, v + 32);
+          loaded(c0 + 64 == kCols);
+          if constexpr (std::is_same<OUT, float>::value) {
+            if (gr < p.m[0]) {
+              if (p.ldy % 4 == 0 && col + 64 <= p.n[0] && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
+#pragma unroll
+                for (int e = 0; e < 64; e += 4)
+                  *reinterpret_cast<float4*>(yr + col + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                  if (col + e < p.n[0]) yr[col + e] = v[e];
+              }
+            }
+          } else {
+            if (leader && p.y_tma) bulk_wait_read();
+            group_sync(bar_id, kBarThreads);
+#pragma unroll
+            for (int c = 0; c < 64; c += 8) {
+              uint4 u;
+              u.x = pack2<T>(v[c], v[c + 1]);
+              u.y = pack2<T>(v[c + 2], v[c + 3]);
+              u.z = pack2<T>(v[c + 4], v[c + 5]);
+              u.w = pack2<T>(v[c + 6], v[c + 7]);
+              *out_piece(grp, c >> 3) = u;
+            }
+            if (p.y_tma) {
+              fence_async_smem();
+              group_sync(bar_id, kBarThreads);
+              if (leader && col < p.n[0]) {
+                tma_store_3d(&p.out[0], base + out_off + grp * kTileA, col, t.m0, 0);
+                bulk_commit();
+              }
+            } else {
+              // rows that TMA cannot address: a warp writes one row at a time, two columns a lane
+              group_sync(bar_id, kBarThreads);
+              const int c = col + 2 * lane;
+              for (int r = wq; r < 128 && t.m0 + r < p.m[0]; r += 4) {
+                const uint32_t u = *reinterpret_cast<const uint32_t*>(
+                    gbase + out_off + grp * kTileA + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
+                uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + ((int64_t)t.m0 + r) * p.ldy + c;
+                if (c < p.n[0]) dst[0] = (uint16_t)u;
+                if (c + 1 < p.n[0]) dst[1] = (uint16_t)(u >> 16);
+              }
+            }
+          }
+        }
+      } else {
+        // fp32 partial sums
+        const int64_t n = p.n[t.job], gr = (int64_t)t.m0 + row;
+        int64_t off = (int64_t)t.split * p.partial_stride;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (j < t.job) off += p.m[j] * p.n[j];
+        float* dst = p.partials + off + gr * n;
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 32) {
+          const int col = t.n0 + grp * kCols + c0;
+          float v[32];
+          columns(0, c0, v);
+          loaded(c0 + 32 == kCols);
+          if (none) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          }
+          if (gr < p.m[t.job]) {
+            if (n % 4 == 0 && col + 32 <= n) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                float4* q = reinterpret_cast<float4*>(dst + col + e);
+                float4 u = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                if (p.add) {
+                  const float4 o = *q;
+                  u = make_float4(u.x + o.x, u.y + o.y, u.z + o.z, u.w + o.w);
+                }
+                *q = u;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (col + e < n) dst[col + e] = p.add ? dst[col + e] + v[e] : v[e];
+            }
+          }
+        }
+      }
+    }
+    bulk_wait();
+  }
+
+  // -------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000LL) {
+    }
+    if (tid == 0) set_status(p.status, kStatusTimeoutFeedForward);
+    __syncthreads();
+  }
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// `box_cols` x `box_rows` tiles of a matrix
+bool map_of(CUtensorMap* map, bool bf16, const Matrix& m, int box_cols, int box_rows) {
+  const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, (uint64_t)m.planes};
+  const uint64_t st[2] = {(uint64_t)m.pitch * 2, (uint64_t)m.plane * 2};
+  const uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
+  return make_tensor_map(map, bf16, 3, m.p, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int64_t tiles_of(int64_t x, int tile) { return (x + tile - 1) / tile; }
+
+template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN>
+cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
+  using C = Cfg<MODE, NT>;
+  Params p = {};
+  bool ok = true;
+  int64_t tiles = 0;
+  if (MODE == kWeight) {
+    for (int j = 0; j < 3; ++j) {
+      p.m[j] = g.a[j].cols;
+      p.n[j] = g.b[j].cols;
+      p.k[j] = g.a[j].rows;
+      p.m_tiles[j] = (int)tiles_of(p.m[j], 128);
+      p.n_tiles[j] = (int)tiles_of(p.n[j], NT);
+      tiles += (int64_t)p.m_tiles[j] * p.n_tiles[j] * g.splits;
+      ok = ok && map_of(&p.a[j], g.bf16, g.a[j], 64, kBK) && map_of(&p.b[j], g.bf16, g.b[j], 64, kBK);
+    }
+  } else {
+    p.phases = MODE == kHidden ? 2 : MODE == kLinear ? g.products : 1;
+    p.m[0] = g.a[0].rows;
+    p.n[0] = MODE == kLinear && B_MN ? g.b[0].cols : g.b[0].rows;
+    p.m_tiles[0] = (int)tiles_of(p.m[0], 128);
+    p.n_tiles[0] = (int)tiles_of(p.n[0], NT);
+    tiles = (int64_t)p.m_tiles[0] * p.n_tiles[0];
+    for (int i = 0; i < p.phases; ++i) {
+      p.k[i] = g.a[i].cols;
+      ok = ok && map_of(&p.a[i], g.bf16, g.a[i], kBK, 128);
+    }
+    if (MODE == kLinear) {
+      for (int i = 0; i < p.phases; ++i)
+        ok = ok && (B_MN ? map_of(&p.b[i], g.bf16, g.b[i], 64, kBK) : map_of(&p.b[i], g.bf16, g.b[i], kBK, NT));
+      if (g.y_tma) ok = ok && map_of(&p.out[0], g.bf16, g.out[0], 64, 128);
+    } else {
+      for (int i = 0; i < 2; ++i) ok = ok && map_of(&p.b[i], g.bf16, g.b[i], kBK, NT);
+      if (MODE == kHidden) ok = ok && map_of(&p.b[2], g.bf16, g.b[2], 64, kBK);
+      for (int i = 0; i < (MODE == kHidden ? 3 : 1); ++i) ok = ok && map_of(&p.out[i], g.bf16, g.out[i], 64, 128);
+    }
+  }
+  if (!ok || tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+  if (tiles == 0) return cudaSuccess;
+  p.tiles = (int)tiles;
+  p.y = g.y;
+  p.ldy = g.ldy;
+  p.y_tma = g.y_tma;
+  p.partials = g.partials;
+  p.partial_stride = g.partial_stride;
+  p.splits = g.splits;
+  p.add = g.add;
+  p.status = g.status;
+  constexpr auto kern = ff_gemm_kernel<T, PARTS, OUT, MODE, NT, B_MN>;
+  cudaError_t e = opt_in_smem<kern>(C::smem_bytes());
+  if (e != cudaSuccess) return e;
+  const int sms = sm_count();
+  return launch_early(kern, dim3(p.tiles < sms ? p.tiles : sms), kThreads, C::smem_bytes(), stream, p);
+}
+
+// 256 columns a tile where every result has more than 128 (fp32: 128, for the sums in registers).
+bool wide_tiles(bool f32, std::initializer_list<int64_t> n) {
+  for (int64_t c : n)
+    if (f32 || c <= 128) return false;
+  return true;
+}
+
+template <typename T, int PARTS, typename OUT>
+cudaError_t dispatch(const GemmArgs& g, cudaStream_t s) {
+  constexpr int kWide = PARTS == 3 ? 128 : 256;
+  switch (g.mode) {
+    case kGate: return launch<T, PARTS, OUT, kGate, kWide / 2, false>(g, s);
+    case kHidden: return launch<T, PARTS, OUT, kHidden, 64, false>(g, s);
+    case kLinear: {
+      const bool wide = wide_tiles(PARTS == 3, {g.b_mn ? g.b[0].cols : g.b[0].rows});
+      if (g.b_mn) return wide ? launch<T, PARTS, OUT, kLinear, kWide, true>(g, s) : launch<T, PARTS, OUT, kLinear, 128, true>(g, s);
+      return wide ? launch<T, PARTS, OUT, kLinear, kWide, false>(g, s) : launch<T, PARTS, OUT, kLinear, 128, false>(g, s);
+    }
+    default:
+      return wide_tiles(PARTS == 3, {g.b[0].cols, g.b[1].cols, g.b[2].cols}) ? launch<T, PARTS, OUT, kWeight, kWide, true>(g, s)
+                                                                            : launch<T, PARTS, OUT, kWeight, 128, true>(g, s);
+  }
+}
+
+}  // namespace
+
+cudaError_t gemm(const GemmArgs& g, cudaStream_t s) {
+  if (g.a[0].planes == 3) return dispatch<__nv_bfloat16, 3, float>(g, s);
+  return g.bf16 ? dispatch<__nv_bfloat16, 1, __nv_bfloat16>(g, s) : dispatch<__half, 1, __half>(g, s);
+}
+
+// The number of splits whose rounds of tiles over the SMs cost least (a split's last reads and writes
+// are counted as 1/32 of a round); at least 256 rows a split.
+int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms) {
+  const bool wide = wide_tiles(f32, {n[0], n[1], n[2]});
+  int64_t tiles = 0;
+  for (int j = 0; j < 3; ++j) tiles += tiles_of(m[j], 128) * tiles_of(n[j], wide ? 256 : 128);
+  int best = 1;
+  float cost = 1e30f;
+  for (int s = 1; s <= 32 && (s == 1 || rows / s >= 256); ++s) {
+    const float c = (float)tiles_of(tiles * s, sms) * (1.f / s + 1.f / 32);
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
+}  // namespace ff
+}  // namespace trifast

@@ -1,0 +1,57 @@
+// Host interface of the feed-forward block's matrix products (ff_gemm.cu) and of the kernels around
+// them (ff_support.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace trifast {
+namespace ff {
+
+// A matrix as the products read or write it: `rows` x `cols` 16-bit elements, rows `pitch` elements
+// apart (a multiple of 8), in `planes` planes (1; or 3, the parts of fp32 values, see ff_support.cu),
+// `plane` elements apart.
+struct Matrix {
+  void* p;
+  int64_t rows, cols, pitch;
+  int planes;
+  int64_t plane;
+};
+
+// What is made of the accumulators of a tile.
+enum Mode {
+  kGate,    // h = silu(X Wg^T) * (X Wu^T)
+  kLinear,  // Y = A B^T (+ A1 B1^T)
+  kHidden,  // da, db, h from X Wg^T, X Wu^T and dY Wd
+  kWeight,  // fp32 sums of A^T B over rows, three products in one launch
+};
+
+struct GemmArgs {
+  int mode;
+  bool bf16;         // type of the 16-bit elements
+  bool b_mn;         // kLinear: B is (K, N), N contiguous (else (N, K), K contiguous)
+  int products;      // kLinear: 1 or 2 (their sum)
+  Matrix a[3], b[3]; // kGate: a0 = X, b = Wg, Wu.  kHidden: a0 = X, a1 = dY, b = Wg, Wu, Wd
+  Matrix out[3];     // kGate: h.  kHidden: da, db, h.  (kLinear with a TMA-addressable result: y)
+  // kLinear: the result, in its own type
+  void* y;
+  int64_t ldy;
+  int y_dtype;
+  bool y_tma;        // out[0] describes y
+  // kWeight: partial sums (splits, m0 * n0 + m1 * n1 + m2 * n2) fp32; added to what is there if `add`
+  float* partials;
+  int64_t partial_stride;
+  int splits;
+  bool add;
+  unsigned int* status;
+};
+cudaError_t gemm(const GemmArgs& g, cudaStream_t s);
+// Row splits of a kWeight launch over `rows` rows whose products have m[i] x n[i] results.
+int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms);
+
+// dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of `dtype`)
+cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Matrix& dst, cudaStream_t s);
+// dst[i] = sum over `splits` of partials[split * stride + i], in `dtype`
+cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* dst, int64_t count, int dtype, cudaStream_t s);
+
+}  // namespace ff
+}  // namespace trifast

@@ -1,0 +1,89 @@
+// Kernels around the products of the feed-forward block: operands laid out for them, and the sum of the
+// weight gradients' partial sums.
+
+#include <type_traits>
+
+#include "ff_gemm.cuh"
+#include "tc_common.cuh"
+
+namespace trifast {
+namespace ff {
+namespace {
+
+// A matrix with rows of 16-byte pitch, and fp32 as three bf16 planes.  A value is cut, not rounded, to its
+// upper 8 significant bits, and what is left again: the three parts hold its 24 bits exactly and
+// have one sign.  A thread makes eight columns of a row; rows behind the last are zero.
+template <typename T>
+__global__ void stage_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, Matrix dst) {
+  after_previous();
+  const int64_t per_row = dst.pitch / 8, total = dst.rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per_row, c = (i % per_row) * 8;
+    T v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = r < rows && c + e < dst.cols ? src[r * ld + c + e] : from_f32<T>(0.f);
+    uint16_t* out = reinterpret_cast<uint16_t*>(dst.p) + r * dst.pitch + c;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = __float_as_uint(v[2 * e]), b = __float_as_uint(v[2 * e + 1]);
+          u[e] = __byte_perm(a, b, 0x7632);
+          v[2 * e] -= __uint_as_float(a & 0xffff0000u);
+          v[2 * e + 1] -= __uint_as_float(b & 0xffff0000u);
+        }
+        *reinterpret_cast<uint4*>(out + q * dst.plane) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    } else {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint16_t lo, hi;
+        memcpy(&lo, &v[2 * e], 2);
+        memcpy(&hi, &v[2 * e + 1], 2);
+        u[e] = lo | (uint32_t)hi << 16;
+      }
+      *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+}
+
+// The splits are added in order, in fp32.
+template <typename T>
+__global__ void sum_partials_kernel(const float* __restrict__ partials, int splits, int64_t stride, T* __restrict__ dst, int64_t count) {
+  after_previous();
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += partials[k * stride + i];
+    dst[i] = from_f32<T>(s);
+  }
+}
+
+dim3 grid_for(int64_t threads) {
+  const int64_t b = (threads + 255) / 256, most = (int64_t)sm_count() * 16;
+  return dim3((unsigned)(b < most ? b : most));
+}
+
+}  // namespace
+
+cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Matrix& dst, cudaStream_t s) {
+  const int64_t threads = dst.rows * (dst.pitch / 8);
+  if (threads == 0) return cudaSuccess;
+  if (dtype == TRIFAST_F32) return launch_early(stage_kernel<float>, grid_for(threads), 256, 0, s, (const float*)src, ld, rows, dst);
+  return launch_early(stage_kernel<__half>, grid_for(threads), 256, 0, s, (const __half*)src, ld, rows, dst);
+}
+
+cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* dst, int64_t count, int dtype, cudaStream_t s) {
+  const dim3 g = grid_for(count);
+  switch (dtype) {
+    case TRIFAST_F32: return launch_early(sum_partials_kernel<float>, g, 256, 0, s, partials, splits, stride, (float*)dst, count);
+    case TRIFAST_BF16: return launch_early(sum_partials_kernel<__nv_bfloat16>, g, 256, 0, s, partials, splits, stride, (__nv_bfloat16*)dst, count);
+    default: return launch_early(sum_partials_kernel<__half>, g, 256, 0, s, partials, splits, stride, (__half*)dst, count);
+  }
+}
+
+}  // namespace ff
+}  // namespace trifast

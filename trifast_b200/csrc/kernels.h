@@ -101,6 +101,11 @@ cudaError_t tc_bwd_dqkv_fused(const BwdArgs& a, cudaStream_t s);
 // Sum of the row shards' fp32 db partials by peer stores (db_push_reduce.cu).
 cudaError_t db_push_reduce(const trifast_push_reduce* a, unsigned int* status, cudaStream_t s);
 
+// The current device's status word, or a trifast_status (it has none, or is not a B200).
+int device_status(unsigned int** status);
+// TRIFAST_OK, or TRIFAST_ERR_LAUNCH with the error kept for trifast_last_cuda_error().
+int cuda_rc(cudaError_t e);
+
 // One warp whose bounded wait runs out after limit_cycles (test support).
 cudaError_t wait_probe(long long limit_cycles, unsigned int* status, cudaStream_t s);
 

@@ -21,11 +21,57 @@
 #include <cstdlib>
 #include <cstring>
 
-#include "../../include/trifast_b200.h"
+#include "torch_common.h"
+
+namespace trifast_torch {
+
+int32_t dtype_code(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return TRIFAST_F32;
+    case at::kBFloat16: return TRIFAST_BF16;
+    case at::kHalf: return TRIFAST_F16;
+    default:
+      TORCH_CHECK_TYPE(false, "unsupported dtype ", t, "; expected float32, bfloat16 or float16");
+  }
+}
+
+void check_rc(int rc, const char* what) {
+  if (rc == TRIFAST_OK) return;
+  TORCH_CHECK(false, what, ": ", trifast_status_str(rc), " (status ", rc,
+              rc == TRIFAST_ERR_LAUNCH ? std::string(", ") + trifast_last_cuda_error() : std::string(),
+              ")");
+}
+
+void raise_if_device_gave_up(c10::DeviceIndex dev, cudaStream_t stream) {
+  static std::atomic<volatile uint32_t*> words[64];
+  TORCH_CHECK(dev >= 0 && dev < 64, "device index ", (int)dev);
+  volatile uint32_t* w = words[dev].load(std::memory_order_acquire);
+  if (!w) {
+    uint32_t* p = nullptr;
+    check_rc(trifast_host_status_word(&p), "trifast_host_status_word");
+    w = p;
+    words[dev].store(w, std::memory_order_release);
+  }
+  if (*w == 0) return;
+  // (while the stream is being captured the status cannot be read: the word stays set, and the
+  // next call outside the capture clears both)
+  const bool cleared = trifast_check_device_status(stream) != TRIFAST_ERR_LAUNCH;
+  if (cleared) *w = 0;
+  TORCH_CHECK(false, "trifast_b200: ", trifast_status_str(TRIFAST_ERR_DEVICE_TIMEOUT),
+              " in an earlier call on this device; the results of that call and of the calls "
+              "after it are invalid ",
+              cleared ? "(status cleared, retry is possible)"
+                      : "(the status could not be cleared here, as during a graph capture)");
+}
+
+}  // namespace trifast_torch
 
 namespace {
 
 using at::Tensor;
+using trifast_torch::check_rc;
+using trifast_torch::dtype_code;
+using trifast_torch::raise_if_device_gave_up;
 
 // ------------------------------------------------------------------ arguments
 struct Problem {
@@ -59,16 +105,6 @@ Problem check_inputs(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   check_device("mask", mask);
   TORCH_CHECK(q.is_cuda(), "trifast_b200 runs on CUDA devices only (there is no CPU path)");
   return p;
-}
-
-int32_t dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return TRIFAST_F32;
-    case at::kBFloat16: return TRIFAST_BF16;
-    case at::kHalf: return TRIFAST_F16;
-    default:
-      TORCH_CHECK_TYPE(false, "unsupported dtype ", t, "; expected float32, bfloat16 or float16");
-  }
 }
 
 // A contiguous tensor with the canonical strides: contiguous() alone keeps whatever strides
@@ -148,38 +184,6 @@ trifast_shape make_shape(const Problem& p, const Tensor& b, const Tensor& mask) 
   if (!as_they_lie(b, mask, p.n)) flags |= TRIFAST_FLAG_STRIDED;
   return {(int32_t)p.batch, (int32_t)p.heads, (int32_t)p.n, (int32_t)p.rows, (int32_t)p.d,
           dtype_code(b.scalar_type()), kernel, flags};
-}
-
-void check_rc(int rc, const char* what) {
-  if (rc == TRIFAST_OK) return;
-  TORCH_CHECK(false, what, ": ", trifast_status_str(rc), " (status ", rc,
-              rc == TRIFAST_ERR_LAUNCH ? std::string(", ") + trifast_last_cuda_error() : std::string(),
-              ")");
-}
-
-// First thing in every call: if an earlier kernel on this device gave up on one of its
-// bounded waits, its outputs (and those of every launch since) were never written.  Costs one
-// read of host memory when nothing is wrong.
-void raise_if_device_gave_up(c10::DeviceIndex dev, cudaStream_t stream) {
-  static std::atomic<volatile uint32_t*> words[64];
-  TORCH_CHECK(dev >= 0 && dev < 64, "device index ", (int)dev);
-  volatile uint32_t* w = words[dev].load(std::memory_order_acquire);
-  if (!w) {
-    uint32_t* p = nullptr;
-    check_rc(trifast_host_status_word(&p), "trifast_host_status_word");
-    w = p;
-    words[dev].store(w, std::memory_order_release);
-  }
-  if (*w == 0) return;
-  // (while the stream is being captured the status cannot be read: the word stays set, and the
-  // next call outside the capture clears both)
-  const bool cleared = trifast_check_device_status(stream) != TRIFAST_ERR_LAUNCH;
-  if (cleared) *w = 0;
-  TORCH_CHECK(false, "trifast_b200: ", trifast_status_str(TRIFAST_ERR_DEVICE_TIMEOUT),
-              " in an earlier call on this device; the results of that call and of the calls "
-              "after it are invalid ",
-              cleared ? "(status cleared, retry is possible)"
-                      : "(the status could not be cleared here, as during a graph capture)");
 }
 
 // ------------------------------------------------------------------ CUDA implementations
