@@ -131,6 +131,32 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.gpu
+def test_from_a_thread_that_has_not_used_the_device():
+    """With all memory from the allocator's cache, the first thing such a thread does is to encode a tensor map."""
+    import threading
+
+    from trifast_b200 import gated_feed_forward, triangle_attention
+    x = normal(9600, 64, seed=1, dtype=torch.bfloat16)
+    w = [normal(64, 64, seed=i, dtype=torch.bfloat16) for i in (2, 3, 4)]
+    q, b = normal(1, 2, 64, 64, 32, seed=5, dtype=torch.bfloat16), normal(1, 2, 64, 64, seed=6, dtype=torch.bfloat16)
+    m = torch.zeros(1, 64, 64, dtype=torch.bool, device="cuda")
+    for call in (lambda: gated_feed_forward(x, *w), lambda: triangle_attention(q, q, q, b, m)):
+        want, got = call(), []
+        call()
+
+        def run():
+            try:
+                got.append(call())
+            except Exception as e:   # seen by the assertion below
+                got.append(e)
+        t = threading.Thread(target=run)
+        t.start()
+        t.join()
+        assert isinstance(got[0], torch.Tensor), got[0]
+        assert torch.equal(got[0], want)
+
+
+@pytest.mark.gpu
 def test_gradients_have_no_gradient():
     from trifast_b200 import gated_feed_forward, layer_norm
     x = normal(4, 8, seed=1).requires_grad_()

@@ -84,6 +84,28 @@ def test_sizes(rows, c, h, o, dtype):
     check(*draw(rows, c, h, o, dtype))
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("rows,c,h,o", [
+    (9472, 128, 512, 128), (9601, 128, 64, 128), (18945, 128, 130, 40), (20011, 40, 200, 128), (40003, 128, 64, 128),
+    (38017, 64, 256, 64), (9999, 64, 70, 24), (37889, 100, 290, 100), (12001, 8, 8, 8), (57000, 128, 384, 128),
+])
+def test_rows_of_up_to_128_elements(rows, c, h, o, dtype):
+    """The kernels that keep the hidden values on chip: one and two row tiles to an item, one chunk of hidden units
+    and several, ragged ends of everything."""
+    check(*draw(rows, c, h, o, dtype))
+
+
+def test_sums_of_many_rows_in_one_block():
+    """More row tiles to one block than a run of sums holds."""
+    check(*draw(66001, 16, 4737, 16, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_padded_rows_in_chunks(dtype):
+    """Rows that have to be laid out anew, of more than one chunk, by the kernels that keep the hidden values on chip."""
+    check(*draw(400001, 33, 40, 33, dtype))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("c,h", [(64, 128), (192, 320)])
 def test_many_rows(c, h, dtype):
@@ -118,7 +140,10 @@ def test_gate_far_from_zero(dtype):
     y = gated_feed_forward(x, one, one / 1024, one)
     a = x.double()
     want = a * torch.sigmoid(a) * a / 1024
-    assert_bounded(y, want, 2.5 * U[dtype] * want.abs() + 2.0 ** -20 * want.abs() + 1e-30, "y")
+    # 16-bit types count a gate below -43 as -43: silu of either is negative and not below -43 / (1 + e^43) >
+    # -43 2^-62, so that they differ by less than that, times b = a / 1024
+    far = 0 if dtype == torch.float32 else 43 * 2.0 ** -62 * (a / 1024).abs()
+    assert_bounded(y, want, 2.5 * U[dtype] * want.abs() + 2.0 ** -20 * want.abs() + 1.01 * far + 1e-30, "y")
 
 
 def test_nonfinite_rows_stay_in_their_rows():
@@ -172,6 +197,10 @@ def test_rows_do_not_depend_on_their_neighbours():
     for i in (0, 127, 128, 399):
         assert torch.equal(gated_feed_forward(x[i:i + 1], *w), y[i:i + 1])
     assert torch.equal(gated_feed_forward(x[37:], *w), y[37:])
+    # nor on how many there are
+    many = normal(40000, 128, seed=8, dtype=torch.bfloat16)
+    many[:400] = x
+    assert torch.equal(gated_feed_forward(many, *w)[:400], y)
 
 
 def test_gradient_against_differences():

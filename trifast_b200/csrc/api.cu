@@ -42,6 +42,13 @@ int device_setup(int* dev_out, unsigned int** status) {
   });
   if (!g_status_ptr[dev]) return TRIFAST_ERR_LAUNCH;
   if (g_arch_major[dev] != 10) return TRIFAST_ERR_ARCH;
+  // A host thread that has not used the device yet (autograd's, if all memory came from a cache) has no
+  // current context, without which the driver refuses to encode a tensor map.
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return TRIFAST_ERR_LAUNCH;
+    bound = dev;
+  }
   *dev_out = dev;
   *status = g_status_ptr[dev];
   return TRIFAST_OK;

@@ -6,7 +6,7 @@
 #include <initializer_list>
 
 #include "block_kernels.h"
-#include "ff_gemm.cuh"
+#include "ff_fused.cuh"
 #include "kernels.h"
 
 namespace trifast {
@@ -80,6 +80,7 @@ constexpr int64_t kChunkBytes = 48 << 20;
 
 // The workspace of a call, carved in the order of the members.
 struct FfPlan {
+  bool fused;                              // by the kernels that keep the hidden values on chip
   int planes;
   int64_t pitch_c, pitch_h, pitch_o;       // rows of staged operands and hidden values
   bool stage_c, stage_h, stage_x, stage_dy;  // the operands of that width have to be laid out anew
@@ -89,9 +90,14 @@ struct FfPlan {
   size_t wg, wu, wd, x, dy, h, da, db, partials, total;
 };
 
+// Rows from which on the fused kernels, which have one tile of 128 rows to a multiprocessor, are faster than
+// products that are split over the hidden units, too.
+constexpr int64_t kFusedRows = 148 * 64;
+
 FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
   FfPlan p = {};
   const bool f32 = f->dtype == TRIFAST_F32;
+  p.fused = !f32 && f->width <= ff::kFusedWidth && f->width_out <= ff::kFusedWidth && f->rows >= kFusedRows;
   p.planes = f32 ? 3 : 1;
   p.pitch_c = round_up(f->width, 8);
   p.pitch_h = round_up(f->hidden, 8);
@@ -101,10 +107,10 @@ FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
   p.stage_x = f32 || (f->rows > 1 && f->ld_x % 8);
   p.stage_dy = f32 || (f->rows > 1 && f->ld_dy % 8);
   const int64_t one = 2 * p.planes;
-  int64_t per_row = p.pitch_h * one * (backward ? 3 : 1);
+  int64_t per_row = p.fused ? 0 : p.pitch_h * one * (backward ? 3 : 1);
   if (p.stage_x) per_row += p.pitch_c * one;
   if (backward && p.stage_dy) per_row += p.pitch_o * one;
-  int64_t most = kChunkBytes / per_row / 128 * 128;
+  int64_t most = per_row ? kChunkBytes / per_row / 128 * 128 : (int64_t)1 << 30;
   if (most < 1024) most = 1024;
   const int64_t chunks = (f->rows + most - 1) / most;
   p.chunk = chunks <= 1 ? round_up(f->rows, 128) : round_up((f->rows + chunks - 1) / chunks, 128);
@@ -119,13 +125,14 @@ FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
   p.wd = take(p.stage_h, f->width_out * p.pitch_h * one);
   p.x = take(p.stage_x, p.chunk * p.pitch_c * one);
   p.dy = take(backward && p.stage_dy, p.chunk * p.pitch_o * one);
-  p.h = take(true, p.chunk * p.pitch_h * one);
-  p.da = take(backward, p.chunk * p.pitch_h * one);
-  p.db = take(backward, p.chunk * p.pitch_h * one);
+  p.h = take(!p.fused, p.chunk * p.pitch_h * one);
+  p.da = take(backward && !p.fused, p.chunk * p.pitch_h * one);
+  p.db = take(backward && !p.fused, p.chunk * p.pitch_h * one);
   if (backward && weights) {
     const int64_t m[3] = {f->hidden, f->hidden, f->width_out}, n[3] = {f->width, f->width, f->hidden};
     // (the plan is the same on every device: 148 multiprocessors)
-    p.splits = ff::weight_splits(m, n, f->rows < p.chunk ? f->rows : p.chunk, f32, 148);
+    const int64_t rows = f->rows < p.chunk ? f->rows : p.chunk;
+    p.splits = p.fused ? ff::fused_weight_splits(rows, f->hidden, 148) : ff::weight_splits(m, n, rows, f32, 148);
     p.partial_stride = round_up(f->hidden * (2 * (int64_t)f->width + f->width_out), 4);
     p.partials = take(true, p.splits * p.partial_stride * 4);
   }
@@ -167,13 +174,22 @@ int ff_rows(const trifast_ff* f, const FfPlan& p, bool staged, const void* src, 
   return cuda_rc(ff::stage(from, ld, rows, f->dtype, *m, s));
 }
 
-// Y = A B^T (+ A1 B1^T) into rows of `cols` elements of the call's type.
-void ff_result(const trifast_ff* f, void* dst, int64_t r0, int64_t rows, int64_t cols, ff::GemmArgs* g) {
+ff::FusedArgs fused_args(const trifast_ff* f, const FfWeights& w, const Matrix& x, unsigned int* status) {
+  ff::FusedArgs g = {};
+  g.bf16 = f->dtype != TRIFAST_F16;
+  g.x = x;
+  g.wg = w.gate;
+  g.wu = w.up;
+  g.wd = w.down;
+  g.status = status;
+  return g;
+}
+
+// Rows [r0, r0 + rows) of y or dx, and whether TMA can write them.
+Matrix ff_result(const trifast_ff* f, void* dst, int64_t r0, int64_t rows, int64_t cols, bool* tma) {
   char* y = reinterpret_cast<char*>(dst) + (size_t)r0 * cols * elem(f->dtype);
-  g->y = y;
-  g->ldy = cols;
-  g->y_tma = f->dtype != TRIFAST_F32 && (cols % 8 == 0 || rows == 1) && aligned(y, 16);
-  g->out[0] = Matrix{y, rows, cols, cols, 1, rows * cols};
+  *tma = f->dtype != TRIFAST_F32 && (cols % 8 == 0 || rows == 1) && aligned(y, 16);
+  return Matrix{y, rows, cols, cols, 1, rows * cols};
 }
 
 }  // namespace
@@ -258,6 +274,13 @@ int trifast_feed_forward(const trifast_ff* f, const void* x, const void* w_gate,
     const int64_t rows = f->rows - r0 < p.chunk ? f->rows - r0 : p.chunk;
     Matrix mx;
     if ((rc = ff_rows(f, p, p.stage_x, x, f->ld_x, r0, rows, f->width, p.pitch_c, ws + p.x, &mx, s))) return rc;
+    if (p.fused) {
+      ff::FusedArgs g = fused_args(f, w, mx, status);
+      g.what = ff::kForward;
+      g.out = ff_result(f, y, r0, rows, f->width_out, &g.y_tma);
+      if ((rc = cuda_rc(ff::fused(g, s)))) return rc;
+      continue;
+    }
     const Matrix mh{ws + p.h, rows, f->hidden, p.pitch_h, p.planes, p.chunk * p.pitch_h};
     ff::GemmArgs g = {};
     g.mode = ff::kGate;
@@ -272,7 +295,7 @@ int trifast_feed_forward(const trifast_ff* f, const void* x, const void* w_gate,
     g.products = 1;
     g.a[0] = mh;
     g.b[0] = w.down;
-    ff_result(f, y, r0, rows, f->width_out, &g);
+    g.out[0] = ff_result(f, y, r0, rows, f->width_out, &g.y_tma);
     if ((rc = cuda_rc(ff::gemm(g, s)))) return rc;
   }
   return TRIFAST_OK;
@@ -310,6 +333,24 @@ int trifast_feed_forward_backward(const trifast_ff* f, const void* dy, const voi
     if ((rc = ff_rows(f, p, p.stage_x, x, f->ld_x, r0, rows, f->width, p.pitch_c, ws + p.x, &mx, s)) ||
         (rc = ff_rows(f, p, p.stage_dy, dy, f->ld_dy, r0, rows, f->width_out, p.pitch_o, ws + p.dy, &mdy, s)))
       return rc;
+    if (p.fused) {
+      ff::FusedArgs g = fused_args(f, w, mx, status);
+      g.dy = mdy;
+      if (dx) {
+        g.what = ff::kDx;
+        g.out = ff_result(f, dx, r0, rows, f->width, &g.y_tma);
+        if ((rc = cuda_rc(ff::fused(g, s)))) return rc;
+      }
+      if (weights) {
+        g.what = ff::kDw;
+        g.partials = partials;
+        g.partial_stride = p.partial_stride;
+        g.splits = p.splits;
+        g.add = r0 > 0;
+        if ((rc = cuda_rc(ff::fused(g, s)))) return rc;
+      }
+      continue;
+    }
     auto hidden = [&](size_t off) { return Matrix{ws + off, rows, f->hidden, p.pitch_h, p.planes, p.chunk * p.pitch_h}; };
     const Matrix mda = hidden(p.da), mdb = hidden(p.db), mh = hidden(p.h);
     ff::GemmArgs g = {};
@@ -331,7 +372,7 @@ int trifast_feed_forward_backward(const trifast_ff* f, const void* dy, const voi
       g.products = 2;
       g.a[0] = mda;
       g.a[1] = mdb;
-      ff_result(f, dx, r0, rows, f->width, &g);
+      g.out[0] = ff_result(f, dx, r0, rows, f->width, &g.y_tma);
       if ((rc = cuda_rc(ff::gemm(g, s)))) return rc;
     }
     if (weights) {

@@ -1,0 +1,147 @@
+// Device helpers of the feed-forward block's kernels (ff_gemm.cu, ff_fused.cu) and the tensor maps of their operands.
+#pragma once
+
+#include "ff_gemm.cuh"
+#include "tc_common.cuh"
+
+namespace trifast {
+namespace ff {
+using namespace tc;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+// The same tile as tma_load_3d's into L2 alone.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// A barrier of `threads` threads that tells whether all of them came with `ok`.
+__device__ __forceinline__ bool group_all(int id, int threads, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void group_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + e^-a): 0 and 1 at the ends, NaN for NaN
+__device__ __forceinline__ float sigmoid(float a) { return rcp(1.f + ex2(-kLog2e * a)); }
+
+// The same for two units of a 16-bit call, with less of the special-function unit, which bounds these kernels (16
+// results a cycle and multiprocessor for ex2 and rcp together).  One reciprocal serves both units,
+// 1/u = v / (u v); gates below -43 count as -43 (clamp_gate), where silu is 1e-17, so that u v stays finite.
+// POLY: 2^t by a polynomial, 2^n p(t - n) with n = round(t) and p of degree 4 (relative error 2.7e-6, fitted here
+// for the smallest largest relative error on [-1/2, 1/2]), on the FMA pipe.  A NaN in one unit makes both NaN,
+// and a row with a NaN unit is NaN anyway.
+__device__ __forceinline__ float clamp_gate(float a) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(-43.f));
+  return r;
+}
+template <bool POLY>
+__device__ __forceinline__ void sigmoid2(float a0, float a1, float& s0, float& s1) {
+  float t0, t1, e0, e1;
+  fmul2(t0, t1, a0, a1, -kLog2e, -kLog2e);
+  if constexpr (POLY) {
+    constexpr float kRound = 12582912.f;   // 1.5 2^23: adding it rounds to a whole number, in the low bits
+    t0 = fmaxf(t0, -120.f);
+    t1 = fmaxf(t1, -120.f);
+    float z0, z1, f0, f1;
+    fadd2(z0, z1, t0, t1, kRound, kRound);
+    fadd2(f0, f1, z0, z1, -kRound, -kRound);
+    ffma2(f0, f1, f0, f1, -1.f, -1.f, t0, t1);
+    ffma2(e0, e1, f0, f1, 0.00957053154706955f, 0.00957053154706955f, 0.05591866374015808f, 0.05591866374015808f);
+    ffma2(e0, e1, e0, e1, f0, f1, 0.24024735391139984f, 0.24024735391139984f);
+    ffma2(e0, e1, e0, e1, f0, f1, 0.6931216716766357f, 0.6931216716766357f);
+    ffma2(e0, e1, e0, e1, f0, f1, 0.9999992847442627f, 0.9999992847442627f);
+    e0 = __int_as_float(__float_as_int(e0) + (__float_as_int(z0) << 23));
+    e1 = __int_as_float(__float_as_int(e1) + (__float_as_int(z1) << 23));
+  } else {
+    e0 = ex2(t0);
+    e1 = ex2(t1);
+  }
+  fadd2(e0, e1, e0, e1, 1.f, 1.f);
+  const float r = rcp(e0 * e1);
+  s0 = r * e1;
+  s1 = r * e0;
+}
+
+// h = silu(a) b of N units, packed.  Every other pair by the polynomial.
+template <typename T, int N>
+__device__ __forceinline__ void gate_units(const float* a, const float* b, uint32_t* h) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    const float a0 = clamp_gate(a[e]), a1 = clamp_gate(a[e + 1]);
+    float s0, s1;
+    if (e & 2)
+      sigmoid2<true>(a0, a1, s0, s1);
+    else
+      sigmoid2<false>(a0, a1, s0, s1);
+    fmul2(s0, s1, a0, a1, s0, s1);
+    fmul2(s0, s1, s0, s1, b[e], b[e + 1]);
+    h[e >> 1] = pack2<T>(s0, s1);
+  }
+}
+
+// da = dh b silu'(a), db = dh silu(a) (and h) of N units, packed.
+template <typename T, int N, bool H>
+__device__ __forceinline__ void grad_units(const float* a, const float* b, const float* dh, uint32_t* da, uint32_t* db, uint32_t* h) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    const float a0 = clamp_gate(a[e]), a1 = clamp_gate(a[e + 1]);
+    float s0, s1, v0, v1, w0, w1, q0, q1, r0, r1;
+    if (e & 2)
+      sigmoid2<true>(a0, a1, s0, s1);
+    else
+      sigmoid2<false>(a0, a1, s0, s1);
+    fmul2(v0, v1, a0, a1, s0, s1);                           // silu
+    ffma2(q0, q1, s0, s1, -1.f, -1.f, 1.f, 1.f);
+    ffma2(q0, q1, v0, v1, q0, q1, s0, s1);                   // its slope, s + silu (1 - s)
+    fmul2(w0, w1, dh[e], dh[e + 1], b[e], b[e + 1]);
+    fmul2(w0, w1, w0, w1, q0, q1);
+    fmul2(r0, r1, dh[e], dh[e + 1], v0, v1);
+    da[e >> 1] = pack2<T>(w0, w1);
+    db[e >> 1] = pack2<T>(r0, r1);
+    if constexpr (H) {
+      fmul2(v0, v1, v0, v1, b[e], b[e + 1]);
+      h[e >> 1] = pack2<T>(v0, v1);
+    }
+  }
+}
+
+// `box_cols` x `box_rows` tiles of a matrix
+inline bool map_of(CUtensorMap* map, bool bf16, const Matrix& m, int box_cols, int box_rows) {
+  const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, (uint64_t)m.planes};
+  const uint64_t st[2] = {(uint64_t)m.pitch * 2, (uint64_t)m.plane * 2};
+  const uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
+  return make_tensor_map(map, bf16, 3, m.p, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+}  // namespace ff
+}  // namespace trifast

@@ -23,8 +23,7 @@
 #include <initializer_list>
 #include <type_traits>
 
-#include "ff_gemm.cuh"
-#include "tc_common.cuh"
+#include "ff_device.cuh"
 
 namespace trifast {
 namespace ff {
@@ -35,7 +34,6 @@ constexpr int kBK = 64;                  // contraction per stage
 constexpr int kTileA = 128 * kBK * 2;    // bytes of an operand tile of 128 rows
 constexpr int kThreads = 320;
 constexpr int kSmemLimit = 232448;
-constexpr float kLog2e = 1.4426950408889634f;
 
 // Columns per B matrix (NT), accumulator columns, stages and staging of results by mode.
 template <int MODE, int NT>
@@ -65,59 +63,16 @@ struct Params {
   unsigned int* status;
 };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
-               : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// A barrier of `threads` threads that tells whether all of them came with `ok`.
-__device__ __forceinline__ bool group_all(int id, int threads, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)ok), "r"(id), "r"(threads)
-      : "memory");
-  return r != 0;
-}
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// 1 / (1 + e^-a): 0 and 1 at the ends, NaN for NaN
-__device__ __forceinline__ float sigmoid(float a) { return rcp(1.f + ex2(-kLog2e * a)); }
-
 // Pairs of planes (of A, of B) whose products make up a product of fp32 values, the smallest first.
 __device__ __forceinline__ int plane_a(int q) { return (0x001021 >> (4 * q)) & 15; }   // 1 2 0 1 0 0
 __device__ __forceinline__ int plane_b(int q) { return (0x010201 >> (4 * q)) & 15; }   // 1 0 2 0 1 0
 
-// One part of a value and what is left of it: PARTS = 1 rounds to T, PARTS = 3 cuts to bf16, so that three
-// parts hold all 24 bits.
-template <typename T, int PARTS>
+// One bf16 part of two values, cut and not rounded, and what is left of them: three parts hold all 24 bits.
 __device__ __forceinline__ uint32_t take_part(float& v0, float& v1) {
-  if constexpr (PARTS == 1) {
-    return pack2<T>(v0, v1);
-  } else {
-    const uint32_t a = __float_as_uint(v0), b = __float_as_uint(v1);
-    v0 -= __uint_as_float(a & 0xffff0000u);
-    v1 -= __uint_as_float(b & 0xffff0000u);
-    return __byte_perm(a, b, 0x7632);
-  }
+  const uint32_t a = __float_as_uint(v0), b = __float_as_uint(v1);
+  v0 -= __uint_as_float(a & 0xffff0000u);
+  v1 -= __uint_as_float(b & 0xffff0000u);
+  return __byte_perm(a, b, 0x7632);
 }
 
 // Stages of the largest products that one sum in TMEM takes when PARTS is 3 (those of the smaller ones, five
@@ -419,15 +374,20 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         }
       };
       if constexpr (MODE == kGate) {
-        float h[kCols];
+        float h[kCols];               // PARTS = 3; else packed
+        uint32_t packed[kCols / 2];
 #pragma unroll
         for (int c = 0; c < kCols; c += 32) {
           float a[32], b[32];
           columns(0, c, a);
           columns(1, c, b);
           loaded(c + 32 == kCols);
+          if constexpr (PARTS == 1) {
+            gate_units<T, 32>(a, b, packed + c / 2);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) h[c + e] = a[e] * sigmoid(a[e]) * b[e];
+            for (int e = 0; e < 32; ++e) h[c + e] = a[e] * sigmoid(a[e]) * b[e];
+          }
         }
         const int tile = kShared ? 0 : grp, piece = kShared ? grp * (kCols / 8) : 0, col = t.n0 + tile * 64;
 #pragma unroll
@@ -436,12 +396,12 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
           group_sync(bar_id, kBarThreads);
 #pragma unroll
           for (int c = 0; c < kCols; c += 8) {
-            uint4 u;
-            u.x = take_part<T, PARTS>(h[c], h[c + 1]);
-            u.y = take_part<T, PARTS>(h[c + 2], h[c + 3]);
-            u.z = take_part<T, PARTS>(h[c + 4], h[c + 5]);
-            u.w = take_part<T, PARTS>(h[c + 6], h[c + 7]);
-            *out_piece(tile, piece + (c >> 3)) = u;
+            if constexpr (PARTS == 3) {
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) packed[(c + e) >> 1] = take_part(h[c + e], h[c + e + 1]);
+            }
+            const uint32_t* u = packed + c / 2;
+            *out_piece(tile, piece + (c >> 3)) = make_uint4(u[0], u[1], u[2], u[3]);
           }
           fence_async_smem();
           group_sync(bar_id, kBarThreads);
@@ -452,19 +412,24 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         }
       } else if constexpr (MODE == kHidden) {
         static_assert(MODE != kHidden || NT == 64, "result tiles are 64 columns");
-        float r[3][32];
+        float r[3][32];               // PARTS = 3; else packed
+        uint32_t packed[3][16];
         {
           float a[32], b[32], dh[32];
           columns(0, 0, a);
           columns(1, 0, b);
           columns(2, 0, dh);
           loaded(true);
+          if constexpr (PARTS == 1) {
+            grad_units<T, 32, true>(a, b, dh, packed[0], packed[1], packed[2]);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float s = sigmoid(a[e]), u = a[e] * s;
-            r[0][e] = dh[e] * b[e] * fmaf(u, 1.f - s, s);
-            r[1][e] = dh[e] * u;
-            r[2][e] = u * b[e];
+            for (int e = 0; e < 32; ++e) {
+              const float s = sigmoid(a[e]), u = a[e] * s;
+              r[0][e] = dh[e] * b[e] * fmaf(u, 1.f - s, s);
+              r[1][e] = dh[e] * u;
+              r[2][e] = u * b[e];
+            }
           }
         }
 #pragma unroll
@@ -475,12 +440,12 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
           for (int o = 0; o < 3; ++o)
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
-              uint4 u;
-              u.x = take_part<T, PARTS>(r[o][c], r[o][c + 1]);
-              u.y = take_part<T, PARTS>(r[o][c + 2], r[o][c + 3]);
-              u.z = take_part<T, PARTS>(r[o][c + 4], r[o][c + 5]);
-              u.w = take_part<T, PARTS>(r[o][c + 6], r[o][c + 7]);
-              *out_piece(o, (grp * 32 + c) >> 3) = u;
+              if constexpr (PARTS == 3) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) packed[o][(c + e) >> 1] = take_part(r[o][c + e], r[o][c + e + 1]);
+              }
+              const uint32_t* u = packed[o] + c / 2;
+              *out_piece(o, (grp * 32 + c) >> 3) = make_uint4(u[0], u[1], u[2], u[3]);
             }
           fence_async_smem();
           group_sync(bar_id, kBarThreads);
@@ -603,14 +568,6 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
   }
 }
 
-// `box_cols` x `box_rows` tiles of a matrix
-bool map_of(CUtensorMap* map, bool bf16, const Matrix& m, int box_cols, int box_rows) {
-  const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, (uint64_t)m.planes};
-  const uint64_t st[2] = {(uint64_t)m.pitch * 2, (uint64_t)m.plane * 2};
-  const uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
-  return make_tensor_map(map, bf16, 3, m.p, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 int64_t tiles_of(int64_t x, int tile) { return (x + tile - 1) / tile; }
 
 template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN>
@@ -653,8 +610,8 @@ cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
   if (!ok || tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
   if (tiles == 0) return cudaSuccess;
   p.tiles = (int)tiles;
-  p.y = g.y;
-  p.ldy = g.ldy;
+  p.y = g.out[0].p;
+  p.ldy = g.out[0].pitch;
   p.y_tma = g.y_tma;
   p.partials = g.partials;
   p.partial_stride = g.partial_stride;

@@ -31,12 +31,8 @@ struct GemmArgs {
   bool b_mn;         // kLinear: B is (K, N), N contiguous (else (N, K), K contiguous)
   int products;      // kLinear: 1 or 2 (their sum)
   Matrix a[3], b[3]; // kGate: a0 = X, b = Wg, Wu.  kHidden: a0 = X, a1 = dY, b = Wg, Wu, Wd
-  Matrix out[3];     // kGate: h.  kHidden: da, db, h.  (kLinear with a TMA-addressable result: y)
-  // kLinear: the result, in its own type
-  void* y;
-  int64_t ldy;
-  int y_dtype;
-  bool y_tma;        // out[0] describes y
+  Matrix out[3];     // kGate: h.  kHidden: da, db, h.  kLinear: y, in the call's own type
+  bool y_tma;        // TMA can write y
   // kWeight: partial sums (splits, m0 * n0 + m1 * n1 + m2 * n2) fp32; added to what is there if `add`
   float* partials;
   int64_t partial_stride;
