@@ -81,7 +81,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     values are rounded to x's type between the two products (fp16: a hidden value beyond 65504 is infinite),
     and so are their gradients in the backward, which computes the hidden values again instead of keeping
     them: nothing but the arguments is saved, and the workspace of a call does not grow with the number of
-    rows.  16-bit types count a gate below -43, where silu is 1e-17, as -43.  fp32 products are as exact as fp32 sums, but a row with an infinite value in x or a weight gives
+    rows.  fp32 products are as exact as fp32 sums, but a row with an infinite value in x or a weight gives
     NaN there.  Differentiable, once, in all four.
     """
     return _gated_feed_forward(x, w_gate, w_up, w_down)

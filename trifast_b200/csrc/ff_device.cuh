@@ -53,57 +53,24 @@ __device__ __forceinline__ float rcp(float x) {
 // 1 / (1 + e^-a): 0 and 1 at the ends, NaN for NaN
 __device__ __forceinline__ float sigmoid(float a) { return rcp(1.f + ex2(-kLog2e * a)); }
 
-// The same for two units of a 16-bit call, with less of the special-function unit, which bounds these kernels (16
-// results a cycle and multiprocessor for ex2 and rcp together).  One reciprocal serves both units,
-// 1/u = v / (u v); gates below -43 count as -43 (clamp_gate), where silu is 1e-17, so that u v stays finite.
-// POLY: 2^t by a polynomial, 2^n p(t - n) with n = round(t) and p of degree 4 (relative error 2.7e-6, fitted here
-// for the smallest largest relative error on [-1/2, 1/2]), on the FMA pipe.  A NaN in one unit makes both NaN,
-// and a row with a NaN unit is NaN anyway.
-__device__ __forceinline__ float clamp_gate(float a) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(-43.f));
-  return r;
-}
-template <bool POLY>
+// The same of two units, the arithmetic around the approximations packed.
 __device__ __forceinline__ void sigmoid2(float a0, float a1, float& s0, float& s1) {
-  float t0, t1, e0, e1;
-  fmul2(t0, t1, a0, a1, -kLog2e, -kLog2e);
-  if constexpr (POLY) {
-    constexpr float kRound = 12582912.f;   // 1.5 2^23: adding it rounds to a whole number, in the low bits
-    t0 = fmaxf(t0, -120.f);
-    t1 = fmaxf(t1, -120.f);
-    float z0, z1, f0, f1;
-    fadd2(z0, z1, t0, t1, kRound, kRound);
-    fadd2(f0, f1, z0, z1, -kRound, -kRound);
-    ffma2(f0, f1, f0, f1, -1.f, -1.f, t0, t1);
-    ffma2(e0, e1, f0, f1, 0.00957053154706955f, 0.00957053154706955f, 0.05591866374015808f, 0.05591866374015808f);
-    ffma2(e0, e1, e0, e1, f0, f1, 0.24024735391139984f, 0.24024735391139984f);
-    ffma2(e0, e1, e0, e1, f0, f1, 0.6931216716766357f, 0.6931216716766357f);
-    ffma2(e0, e1, e0, e1, f0, f1, 0.9999992847442627f, 0.9999992847442627f);
-    e0 = __int_as_float(__float_as_int(e0) + (__float_as_int(z0) << 23));
-    e1 = __int_as_float(__float_as_int(e1) + (__float_as_int(z1) << 23));
-  } else {
-    e0 = ex2(t0);
-    e1 = ex2(t1);
-  }
-  fadd2(e0, e1, e0, e1, 1.f, 1.f);
-  const float r = rcp(e0 * e1);
-  s0 = r * e1;
-  s1 = r * e0;
+  fmul2(s0, s1, a0, a1, -kLog2e, -kLog2e);
+  fadd2(s0, s1, ex2(s0), ex2(s1), 1.f, 1.f);
+  s0 = rcp(s0);
+  s1 = rcp(s1);
 }
 
-// h = silu(a) b of N units, packed.  Every other pair by the polynomial.
+// h = silu(a) b of N units, packed.  (One reciprocal for two units, 1/u = v / (u v), and every other exponential by a
+// polynomial on the FMA pipe left the special-function unit half idle and the kernels of ff_fused.cu no faster: 344-360 us
+// against 350 forward, 559-586 against 557 for dX.)
 template <typename T, int N>
 __device__ __forceinline__ void gate_units(const float* a, const float* b, uint32_t* h) {
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
-    const float a0 = clamp_gate(a[e]), a1 = clamp_gate(a[e + 1]);
     float s0, s1;
-    if (e & 2)
-      sigmoid2<true>(a0, a1, s0, s1);
-    else
-      sigmoid2<false>(a0, a1, s0, s1);
-    fmul2(s0, s1, a0, a1, s0, s1);
+    sigmoid2(a[e], a[e + 1], s0, s1);
+    fmul2(s0, s1, a[e], a[e + 1], s0, s1);
     fmul2(s0, s1, s0, s1, b[e], b[e + 1]);
     h[e >> 1] = pack2<T>(s0, s1);
   }
@@ -114,13 +81,9 @@ template <typename T, int N, bool H>
 __device__ __forceinline__ void grad_units(const float* a, const float* b, const float* dh, uint32_t* da, uint32_t* db, uint32_t* h) {
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
-    const float a0 = clamp_gate(a[e]), a1 = clamp_gate(a[e + 1]);
     float s0, s1, v0, v1, w0, w1, q0, q1, r0, r1;
-    if (e & 2)
-      sigmoid2<true>(a0, a1, s0, s1);
-    else
-      sigmoid2<false>(a0, a1, s0, s1);
-    fmul2(v0, v1, a0, a1, s0, s1);                           // silu
+    sigmoid2(a[e], a[e + 1], s0, s1);
+    fmul2(v0, v1, a[e], a[e + 1], s0, s1);                   // silu
     ffma2(q0, q1, s0, s1, -1.f, -1.f, 1.f, 1.f);
     ffma2(q0, q1, v0, v1, q0, q1, s0, s1);                   // its slope, s + silu (1 - s)
     fmul2(w0, w1, dh[e], dh[e + 1], b[e], b[e + 1]);

@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
 
 // ------------------------------------------------------------------ dX
 // An item is one row tile; the chunks alternate between two buffers of TMEM, [0, 192) and [192, 384): S and dH, with da
-// over a's first columns and db over b's; dX [384, 384 + CP).
+// over a's columns and db over b's (16 columns of each 32); dX [384, 384 + CP).
 template <typename T, int CP>
 __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_constant__ Params p) {
   using L = Rows<CP>;
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
   if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), i == DX_FREE || (i >= P_READY && i < P_READY + 2) ? 4 : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), i == DX_FREE ? 4 : (i >= P_READY && i < P_READY + 2) ? 8 : 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -436,9 +436,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
         const uint64_t bg = make_smem_desc(gu, kTile, 1024, kSwizzle128), bu = make_smem_desc(gu + kTile / 2, kTile, 1024, kSwizzle128);
         constexpr uint32_t idesc = make_idesc(128, CP, kBf16, false, true);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_ts(tmem + 384, a + k * 8, bg + k * (2048 >> 4), idesc, (c > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) umma_ts(tmem + 384, a + (k >> 1) * 32 + (k & 1) * 8, bg + k * (2048 >> 4), idesc, (c > 0 || k > 0) ? 1u : 0u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_ts(tmem + 384, a + 64 + k * 8, bu + k * (2048 >> 4), idesc, 1u);
+        for (int k = 0; k < 4; ++k) umma_ts(tmem + 384, a + 64 + (k >> 1) * 32 + (k & 1) * 8, bu + k * (2048 >> 4), idesc, 1u);
         umma_commit(sm.bar(P_FREE + (g & 1)));
         umma_commit(sm.bar(GU_EMPTY + g % kGU));
         if (c == n - 1) umma_commit(sm.bar(DX_DONE));
@@ -452,31 +452,37 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
   } else if (warp >= kOutWarp) {
     write_results<T, CP>(p, sm, tmem + 384, DX_DONE, DX_FREE);
   } else {
+    // both warpgroups take half the units of every chunk: its gradients are the longest link of the chain from one
+    // use of a buffer to the next
     const int grp = warp >> 2;
-    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + grp * 192;
-    for (int g = grp; g < total; g += 2) {
-      if (!wait(S_FULL + grp, (g >> 1) & 1)) break;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int g = 0; g < total; ++g) {
+      if (!wait(S_FULL + (g & 1), (g >> 1) & 1)) break;
       tc_fence_after();
+      const uint32_t ts = lanes + (g & 1) * 192;
       float a[2][16], b[2][16], dh[2][16];
       auto load = [&](int i) {
-        tmem_ld16(ts + 16 * i, reinterpret_cast<uint32_t*>(a[i & 1]));
-        tmem_ld16(ts + 64 + 16 * i, reinterpret_cast<uint32_t*>(b[i & 1]));
-        tmem_ld16(ts + 128 + 16 * i, reinterpret_cast<uint32_t*>(dh[i & 1]));
+        const int c = grp * 32 + i * 16;
+        tmem_ld16(ts + c, reinterpret_cast<uint32_t*>(a[i]));
+        tmem_ld16(ts + 64 + c, reinterpret_cast<uint32_t*>(b[i]));
+        tmem_ld16(ts + 128 + c, reinterpret_cast<uint32_t*>(dh[i]));
       };
       load(0);
+      tmem_wait_ld();
+      load(1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {   // 16 units at a time, the next ones on their way
-        tmem_wait_ld();
-        if (i < 3) load(i + 1);
+      for (int i = 0; i < 2; ++i) {
         uint32_t da[8], db[8];
-        grad_units<T, 16, false>(a[i & 1], b[i & 1], dh[i & 1], da, db, nullptr);
-        tmem_st8(ts + 8 * i, da);
-        tmem_st8(ts + 64 + 8 * i, db);
+        grad_units<T, 16, false>(a[i], b[i], dh[i], da, db, nullptr);
+        if (i == 0) tmem_wait_ld();
+        // (over columns of a and b that this warp has read)
+        tmem_st8(ts + grp * 32 + 8 * i, da);
+        tmem_st8(ts + 64 + grp * 32 + 8 * i, db);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(P_READY + grp));
+      if (lane == 0) mbar_arrive(sm.bar(P_READY + (g & 1)));
     }
   }
   finish(sm, warp == kMmaWarp, tmem, p.status);
