@@ -40,9 +40,10 @@ int check_norm(const trifast_norm* n, bool backward) {
   if (n->rows < 0 || n->rows > kMostRows || n->width < 1 || n->width > 1 << 20) return TRIFAST_ERR_SHAPE;
   if (!known_dtype(n->dtype) || (n->affine_dtype != n->dtype && n->affine_dtype != TRIFAST_F32)) return TRIFAST_ERR_DTYPE;
   if (!(n->eps >= 0.f) || !isfinite(n->eps)) return TRIFAST_ERR_SHAPE;
-  if (n->ld_x < n->width || (backward && n->ld_dy < n->width)) return TRIFAST_ERR_STRIDE;
+  for (int64_t ld : {n->ld_x, backward ? n->ld_dy : n->ld_x})
+    if (ld < n->width || (n->rows > 1 && !layer_norm_rows_fit(ld, n->width, n->dtype))) return TRIFAST_ERR_STRIDE;
   // (rows longer than a block's registers are summed 64 to a block along the grid's second dimension)
-  if (n->width > 8192 && n->rows > (int64_t)65535 * 64) return TRIFAST_ERR_TOO_LARGE;
+  if (n->width > 8192 - 7 && n->rows > (int64_t)65535 * 64) return TRIFAST_ERR_TOO_LARGE;
   return TRIFAST_OK;
 }
 

@@ -10,9 +10,12 @@ struct LayerNormArgs {
   void *y, *dx, *dweight, *dbias;       // any of the gradients may be null
   int64_t rows, ld_x, ld_dy;            // rows of x and dy may be further apart than their width
   int width, dtype, affine_dtype;
+  int classes;                          // set by the launcher
   float eps;
   float* partials;                      // layer_norm_workspace_floats()
 };
+// Whether rows `ld` elements apart begin at the same places of 16-byte pieces as dense ones: what the kernels take.
+bool layer_norm_rows_fit(int64_t ld, int width, int dtype);
 // fp32 words of workspace that the gradients of weight and bias need.
 int64_t layer_norm_workspace_floats(int64_t rows, int width, int dtype);
 cudaError_t layer_norm_forward(const LayerNormArgs& a, cudaStream_t s);

@@ -6,9 +6,13 @@
 // inner), shared along mid: a thread makes the words of its eight columns once and walks along mid with
 // them.
 //
-// What bounds it: memory where the mask is shared.
+// A dropped value is cleared bit by bit before the arithmetic, so that nothing of it enters.
+//
+// What bounds it: memory; and the generator's 40 wide products per eight elements where every element has a
+// word of its own.
 
 #include "block_kernels.h"
+#include "tc_common.cuh"
 
 namespace trifast {
 namespace {
@@ -33,104 +37,229 @@ __device__ __forceinline__ Words philox(uint64_t block, uint64_t offset, uint64_
   return {{c0, c1, c2, c3}};
 }
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Piece { T v[VEC]; };
+// Eight words from mask entry `entry` on.
+__device__ __forceinline__ void words8(uint64_t entry, uint64_t offset, uint64_t key, uint32_t* w) {
+  const int skip = (int)(entry % 4);
+  const Words b0 = philox(entry / 4, offset, key), b1 = philox(entry / 4 + 1, offset, key);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = e < 4 ? b0.w[e] : b1.w[e - 4];
+  if (skip) {
+    const Words b2 = philox(entry / 4 + 2, offset, key);
+#pragma unroll
+    for (int s = 0; s < 3; ++s)      // shifted by one word, `skip` times
+      if (s < skip) {
+#pragma unroll
+        for (int e = 0; e < 7; ++e) w[e] = w[e + 1];
+        w[7] = s == 0 ? b2.w[0] : s == 1 ? b2.w[1] : b2.w[2];
+      }
+  }
+}
 
-// A thread: VEC columns of inner (8 elements, or one where they cannot be read whole), `walk` steps of mid.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) dropout_add_kernel(DropoutArgs a, int64_t cols, int64_t mids, int walk) {
-  constexpr int U = 4;   // loads in flight
-  using P = Piece<T, VEC>;
+// Eight elements in 16-byte pieces (one of 16-bit types, two of fp32), and the bits that stay of them.
+template <typename T> constexpr int kPieces = sizeof(T) / 2;
+template <typename T> struct Eight { uint4 v[kPieces<T>]; };
+
+template <typename T>
+__device__ __forceinline__ Eight<T> keep_mask(const uint32_t* w, uint64_t threshold) {
+  uint32_t k[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) k[e] = (uint64_t)w[e] >= threshold ? 0xffffffffu : 0u;
+  Eight<T> m;
+  if constexpr (sizeof(T) == 4) {
+    m.v[0] = make_uint4(k[0], k[1], k[2], k[3]);
+    m.v[1] = make_uint4(k[4], k[5], k[6], k[7]);
+  } else {
+    m.v[0] = make_uint4(__byte_perm(k[0], k[1], 0x5410), __byte_perm(k[2], k[3], 0x5410), __byte_perm(k[4], k[5], 0x5410),
+                        __byte_perm(k[6], k[7], 0x5410));
+  }
+  return m;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& u, float* f) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(u.x);
+    f[1] = __uint_as_float(u.y);
+    f[2] = __uint_as_float(u.z);
+    f[3] = __uint_as_float(u.w);
+  } else {
+    tc::unpack2<T>(u.x, f[0], f[1]);
+    tc::unpack2<T>(u.y, f[2], f[3]);
+    tc::unpack2<T>(u.z, f[4], f[5]);
+    tc::unpack2<T>(u.w, f[6], f[7]);
+  }
+}
+
+// res + (x & mask) scale
+template <typename T, bool RES>
+__device__ __forceinline__ uint4 apply(uint4 x, const uint4& res, const uint4& m, float scale) {
+  constexpr int N = 16 / sizeof(T);
+  x.x &= m.x;
+  x.y &= m.y;
+  x.z &= m.z;
+  x.w &= m.w;
+  float f[N], r[N];
+  unpack<T>(x, f);
+  if (RES) unpack<T>(res, r);
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    if (RES)
+      tc::ffma2(f[e], f[e + 1], f[e], f[e + 1], scale, scale, r[e], r[e + 1]);
+    else
+      tc::fmul2(f[e], f[e + 1], f[e], f[e + 1], scale, scale);
+  }
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else
+    return make_uint4(tc::pack2<T>(f[0], f[1]), tc::pack2<T>(f[2], f[3]), tc::pack2<T>(f[4], f[5]), tc::pack2<T>(f[6], f[7]));
+}
+
+__device__ __forceinline__ uint64_t key_of(const DropoutArgs& a) { return a.seed + (a.seed_ptr ? (uint64_t)*a.seed_ptr : 0); }
+
+// Shared masks whose inner extent is a multiple of eight: a thread has eight columns and `walk` steps of mid, `mids`
+// apart.  Columns run fastest over the threads, then the first `mids` steps of mid, then outer.
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256) dropout_shared_kernel(DropoutArgs a, int64_t cols, int64_t mids, int walk) {
+  constexpr int U = 4, N = kPieces<T>;   // steps in flight
   after_previous();
-  const uint64_t key = a.seed + (a.seed_ptr ? (uint64_t)*a.seed_ptr : 0);
+  const uint64_t key = key_of(a);
   const int64_t total = a.outer * mids * cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    // columns run fastest, then the first `mids` steps of mid, then outer
     const int64_t col = i % cols, om = i / cols, m0 = om % mids, o = om / mids;
-    const uint64_t entry = (uint64_t)(o * a.inner + col * VEC);
-    uint32_t word[VEC];
-    if constexpr (VEC == 8) {
-      if (entry % 4 == 0) {
-        const Words lo = philox(entry / 4, a.offset, key), hi = philox(entry / 4 + 1, a.offset, key);
+    uint32_t w[8];
+    words8((uint64_t)(o * a.inner + col * 8), a.offset, key, w);
+    const Eight<T> mask = keep_mask<T>(w, a.threshold);
+    const int64_t first = (o * a.mid + m0) * a.inner + col * 8, step = mids * a.inner;   // elements
+    const int steps = (int)min((int64_t)walk, (a.mid - m0 + mids - 1) / mids);
+    const T* x = reinterpret_cast<const T*>(a.x) + first;
+    const T* r = reinterpret_cast<const T*>(a.residual) + first;
+    T* y = reinterpret_cast<T*>(a.y) + first;
+    int s = 0;
+    for (; s + U <= steps; s += U, x += U * step, r += U * step, y += U * step) {
+      uint4 vx[U][N], vr[U][N];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) word[e] = e < 4 ? lo.w[e] : hi.w[e - 4];
-      } else {
-        const Words b[3] = {philox(entry / 4, a.offset, key), philox(entry / 4 + 1, a.offset, key), philox(entry / 4 + 2, a.offset, key)};
-        const int skip = (int)(entry % 4);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          word[e] = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (k == skip) word[e] = b[(e + k) / 4].w[(e + k) % 4];
+        for (int k = 0; k < N; ++k) {
+          vx[u][k] = reinterpret_cast<const uint4*>(x + u * step)[k];
+          if (RES) vr[u][k] = reinterpret_cast<const uint4*>(r + u * step)[k];
         }
-      }
-    } else {
-      const Words b = philox(entry / 4, a.offset, key);
-      const int at = (int)(entry % 4);
-      word[0] = at == 0 ? b.w[0] : at == 1 ? b.w[1] : at == 2 ? b.w[2] : b.w[3];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < N; ++k) reinterpret_cast<uint4*>(y + u * step)[k] = apply<T, RES>(vx[u][k], vr[u][k], mask.v[k], a.scale);
     }
-    uint32_t keep = 0;
+    for (; s < steps; ++s, x += step, r += step, y += step) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) keep |= (uint32_t)((uint64_t)word[e] >= a.threshold) << e;
-    for (int w0 = 0; w0 < walk; w0 += U) {
-      P x[U], r[U];
-      int64_t at[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t m = m0 + (int64_t)(w0 + u) * mids;
-        const bool in = w0 + u < walk && m < a.mid;
-        at[u] = in ? (o * a.mid + m) * a.inner + col * VEC : -1;
-        if (in) {
-          x[u] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(a.x) + at[u]);
-          if (a.residual) r[u] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(a.residual) + at[u]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (at[u] < 0) continue;
-        P y;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          // (a dropped value does not enter: not an infinity or NaN either)
-          float v = (keep >> e) & 1 ? to_f32<T>(x[u].v[e]) * a.scale : 0.f;
-          if (a.residual) v += to_f32<T>(r[u].v[e]);
-          y.v[e] = from_f32<T>(v);
-        }
-        *reinterpret_cast<P*>(reinterpret_cast<T*>(a.y) + at[u]) = y;
+      for (int k = 0; k < N; ++k) {
+        const uint4 vr = RES ? reinterpret_cast<const uint4*>(r)[k] : make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(y)[k] = apply<T, RES>(reinterpret_cast<const uint4*>(x)[k], vr, mask.v[k], a.scale);
       }
     }
   }
 }
 
-template <typename T, int VEC>
-cudaError_t launch_vec(const DropoutArgs& a, cudaStream_t s) {
-  const int64_t cols = a.inner / VEC, lanes = a.outer * cols;
-  // Steps of mid that a thread walks with one mask: as many as leave eight blocks of 256 threads a multiprocessor.
-  const int64_t want = (int64_t)sm_count() * 8 * 256;
-  int64_t walk = lanes * a.mid / want;
-  if (walk < 1) walk = 1;
-  if (walk > a.mid) walk = a.mid;
-  if (walk > 64) walk = 64;
-  const int64_t mids = (a.mid + walk - 1) / walk, total = lanes * mids;
-  const int64_t blocks = (total + 255) / 256;
-  return launch_early(dropout_add_kernel<T, VEC>, dim3((unsigned)(blocks < 1 << 30 ? blocks : 1 << 30)), 256, 0, s, a, cols, mids, (int)walk);
+// Every element its own word: the tensor as one row of pieces of eight, two of them a thread at a time; the last
+// elements one by one.
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256) dropout_own_kernel(DropoutArgs a) {
+  constexpr int N = kPieces<T>;
+  after_previous();
+  const uint64_t key = key_of(a);
+  const int64_t pieces = a.inner / 8, stride = (int64_t)gridDim.x * 256;
+  const uint4* x = reinterpret_cast<const uint4*>(a.x);
+  const uint4* r = reinterpret_cast<const uint4*>(a.residual);
+  uint4* y = reinterpret_cast<uint4*>(a.y);
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = i0; i < pieces; i += 2 * stride) {
+    uint4 vx[2][N], vr[2][N];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (i + u * stride < pieces)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          vx[u][k] = x[(i + u * stride) * N + k];
+          if (RES) vr[u][k] = r[(i + u * stride) * N + k];
+        }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (i + u * stride >= pieces) break;
+      const uint64_t block = (uint64_t)(i + u * stride) * 2;
+      const Words lo = philox(block, a.offset, key), hi = philox(block + 1, a.offset, key);
+      const uint32_t w[8] = {lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]};
+      const Eight<T> mask = keep_mask<T>(w, a.threshold);
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[(i + u * stride) * N + k] = apply<T, RES>(vx[u][k], vr[u][k], mask.v[k], a.scale);
+    }
+  }
+  if (i0 < a.inner % 8) {
+    const int64_t e = pieces * 8 + i0;
+    const Words b = philox((uint64_t)e / 4, a.offset, key);
+    const int at = (int)(e % 4);
+    const uint32_t w = at == 0 ? b.w[0] : at == 1 ? b.w[1] : at == 2 ? b.w[2] : b.w[3];
+    const float v = (uint64_t)w >= a.threshold ? to_f32<T>(reinterpret_cast<const T*>(a.x)[e]) : 0.f;
+    reinterpret_cast<T*>(a.y)[e] =
+        from_f32<T>(RES ? fmaf(v, a.scale, to_f32<T>(reinterpret_cast<const T*>(a.residual)[e])) : v * a.scale);
+  }
 }
 
-template <typename T>
-cudaError_t launch_type(const DropoutArgs& a, cudaStream_t s) {
-  constexpr uintptr_t kBytes = 8 * sizeof(T);
-  auto whole = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & (kBytes - 1)) == 0; };
-  if (a.inner % 8 == 0 && whole(a.x) && whole(a.residual) && whole(a.y)) return launch_vec<T, 8>(a, s);
-  return launch_vec<T, 1>(a, s);
+// Shared masks of other inner extents: a thread has one column.
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256) dropout_column_kernel(DropoutArgs a, int64_t mids, int walk) {
+  after_previous();
+  const uint64_t key = key_of(a);
+  const int64_t total = a.outer * mids * a.inner;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t col = i % a.inner, om = i / a.inner, m0 = om % mids, o = om / mids;
+    const uint64_t entry = (uint64_t)(o * a.inner + col);
+    const Words b = philox(entry / 4, a.offset, key);
+    const int at = (int)(entry % 4);
+    const uint32_t w = at == 0 ? b.w[0] : at == 1 ? b.w[1] : at == 2 ? b.w[2] : b.w[3];
+    const bool keep = (uint64_t)w >= a.threshold;
+    int64_t e = (o * a.mid + m0) * a.inner + col;
+#pragma unroll 4
+    for (int64_t m = m0; m < a.mid; m += mids, e += mids * a.inner) {
+      const float v = keep ? to_f32<T>(reinterpret_cast<const T*>(a.x)[e]) : 0.f;
+      reinterpret_cast<T*>(a.y)[e] =
+          from_f32<T>(RES ? fmaf(v, a.scale, to_f32<T>(reinterpret_cast<const T*>(a.residual)[e])) : v * a.scale);
+    }
+  }
+}
+
+unsigned blocks_for(int64_t threads, int64_t most) {
+  const int64_t b = (threads + 255) / 256;
+  return (unsigned)(b < most ? b : most);
+}
+
+template <typename T, bool RES>
+cudaError_t launch_type(DropoutArgs a, cudaStream_t s) {
+  const int64_t sms = sm_count();
+  if (a.mid == 1) {   // (no entry has two elements)
+    a.inner *= a.outer;
+    a.outer = 1;
+    const int64_t threads = a.inner / 16 > a.inner % 8 ? a.inner / 16 : a.inner % 8;
+    return launch_early(dropout_own_kernel<T, RES>, dim3(blocks_for(threads < 1 ? 1 : threads, sms * 8)), 256, 0, s, a);
+  }
+  const bool whole = a.inner % 8 == 0;
+  const int64_t cols = whole ? a.inner / 8 : a.inner, lanes = a.outer * cols;
+  // Steps of mid that a thread walks with one mask: as many as leave eight blocks of 256 threads a multiprocessor.
+  int64_t walk = lanes * a.mid / (sms * 8 * 256);
+  walk = walk < 1 ? 1 : walk > 64 ? 64 : walk;
+  if (walk > a.mid) walk = a.mid;
+  const int64_t mids = (a.mid + walk - 1) / walk;
+  const unsigned blocks = blocks_for(lanes * mids, 1 << 30);
+  if (whole) return launch_early(dropout_shared_kernel<T, RES>, dim3(blocks), 256, 0, s, a, cols, mids, (int)walk);
+  return launch_early(dropout_column_kernel<T, RES>, dim3(blocks), 256, 0, s, a, mids, (int)walk);
 }
 
 }  // namespace
 
 cudaError_t dropout_add(const DropoutArgs& a, cudaStream_t s) {
+  const bool r = a.residual != nullptr;
   switch (a.dtype) {
-    case TRIFAST_F32: return launch_type<float>(a, s);
-    case TRIFAST_BF16: return launch_type<__nv_bfloat16>(a, s);
-    default: return launch_type<__half>(a, s);
+    case TRIFAST_F32: return r ? launch_type<float, true>(a, s) : launch_type<float, false>(a, s);
+    case TRIFAST_BF16: return r ? launch_type<__nv_bfloat16, true>(a, s) : launch_type<__nv_bfloat16, false>(a, s);
+    default: return r ? launch_type<__half, true>(a, s) : launch_type<__half, false>(a, s);
   }
 }
 

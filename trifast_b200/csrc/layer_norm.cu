@@ -2,52 +2,55 @@
 //     mu = mean(x),  r = (mean((x - mu)^2) + eps)^-1/2,  xh = (x - mu) r,  y = xh w + b
 //     g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum over rows of dy xh,  db = sum of dy
 //
-// A row lies in the registers of TPR threads (8, 16 or 32 lanes of a warp, or a whole block), E elements
-// each, so that x is read once, its variance is that of the deviations from the mean, and the backward
-// makes both again from x instead of reading them (8 bytes a row less, for two more reductions, which the
-// memory hides).  A thread has the same columns in all of its rows: w and b stay in registers, and so do
-// its sums for dw and db, which meet in shared memory, then as one partial row a block, and are summed in a
-// fixed order by a second kernel.  All arithmetic is in fp32; every result is rounded once.
+// A row lies in the registers of TPR threads (4 to 32 lanes of a warp, or a whole block), up to 16 elements each, so
+// that x is read once, its variance is that of the deviations from the mean, and the backward makes both again
+// from x instead of reading them (8 bytes a row less).  Two sums at a time go around: mean(x) with mean(g), which does
+// not need it; then the variance with sum(g (x - mu)).  A thread has the same columns in all of its rows: w and
+// b stay in registers, and so do its sums for dw and db, which meet in shared memory, then as one partial row a
+// block, and are summed in a fixed order by a second kernel.  All arithmetic is in fp32; every result is rounded once.
 //
-// What bounds it: memory.  Rows whose bytes are no multiple of 16 are read element by element; rows beyond
-// 8192 elements (kMaxRow) are walked in passes instead.
+// Rows whose bytes are no multiple of 16 (SHIFT) are read in the 16-byte pieces that they lie in all the same: rows of
+// one class modulo 8 (fp32: 4) begin at the same place of a piece, and a block takes rows of one class, so that its
+// threads keep their columns.  What a piece holds of other rows is set to zero.
+//
+// What bounds it: memory.  Rows beyond 8192 elements (kMaxRow) are walked in passes instead.
 
 #include <type_traits>
 
 #include "block_kernels.h"
+#include "tc_common.cuh"
 
 namespace trifast {
 namespace {
 
-constexpr int kMaxRow = 8192;
+constexpr int kMaxRow = 8192;   // elements, with those of its first piece that are not its own
 
-template <typename T, int VEC> struct Raw;
-template <typename T> struct Raw<T, 1> { T v; };
-template <> struct Raw<float, 4> { uint4 v; };
-template <> struct Raw<__nv_bfloat16, 8> { uint4 v; };
-template <> struct Raw<__half, 8> { uint4 v; };
+using tc::fadd2;
+using tc::ffma2;
+using tc::fmul2;
 
-template <typename T, int VEC>
-__device__ __forceinline__ void unpack(const Raw<T, VEC>& r, float* f) {
-  T t[VEC];
-  memcpy(t, &r, sizeof(t));
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) f[e] = to_f32<T>(t[e]);
+// A 16-byte piece of a row.
+template <typename T> constexpr int kVec = 16 / sizeof(T);
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& r, float* f) {
+  if constexpr (std::is_same<T, float>::value) {
+    f[0] = __uint_as_float(r.x);
+    f[1] = __uint_as_float(r.y);
+    f[2] = __uint_as_float(r.z);
+    f[3] = __uint_as_float(r.w);
+  } else {
+    tc::unpack2<T>(r.x, f[0], f[1]);
+    tc::unpack2<T>(r.y, f[2], f[3]);
+    tc::unpack2<T>(r.z, f[4], f[5]);
+    tc::unpack2<T>(r.w, f[6], f[7]);
+  }
 }
-template <typename T, int VEC>
-__device__ __forceinline__ Raw<T, VEC> pack(const float* f) {
-  T t[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) t[e] = from_f32<T>(f[e]);
-  Raw<T, VEC> r;
-  memcpy(&r, t, sizeof(t));
-  return r;
-}
-template <typename T, int VEC>
-__device__ __forceinline__ Raw<T, VEC> zero_raw() {
-  Raw<T, VEC> r;
-  memset(&r, 0, sizeof(r));
-  return r;
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float* f) {
+  if constexpr (std::is_same<T, float>::value)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else
+    return make_uint4(tc::pack2<T>(f[0], f[1]), tc::pack2<T>(f[2], f[3]), tc::pack2<T>(f[4], f[5]), tc::pack2<T>(f[6], f[7]));
 }
 
 __device__ __forceinline__ float affine_at(const void* p, int dtype, int i) {
@@ -85,172 +88,238 @@ __device__ __forceinline__ void row_sums(float* v, float (*buf)[32]) {
 
 template <int TPR> constexpr int kBlock = TPR > 32 ? TPR : 256;
 
-// Where a thread's elements lie: piece k at column (k * TPR + lane) * VEC.
-template <int TPR, int VEC>
-__device__ __forceinline__ int col_of(int lane, int k) { return (k * TPR + lane) * VEC; }
+// The pieces of a row that a thread has: piece k begins at column (k * TPR + lane) * VEC - shift.
+template <typename T, int TPR, int K, bool SHIFT>
+struct RowPieces {
+  static constexpr int VEC = kVec<T>, E = K * VEC;
+  int lane, width, shift;
+  int64_t rows;
 
-template <typename T, int VEC, int K>
-__device__ __forceinline__ void load_row(Raw<T, VEC>* r, const T* p, bool valid, int width, int lane, int tpr) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (k * tpr + lane) * VEC;
-    r[k] = valid && c < width ? *reinterpret_cast<const Raw<T, VEC>*>(p + c) : zero_raw<T, VEC>();
+  __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * VEC - (SHIFT ? shift : 0); }
+  __device__ __forceinline__ bool any(int k) const { return col(k) < width; }
+  __device__ __forceinline__ bool has(int k, int e) const {
+    return SHIFT ? (unsigned)(col(k) + e) < (unsigned)width : any(k);
   }
-}
-
-// Mean and 1 / standard deviation of R rows.
-template <typename T, int VEC, int TPR, int K, int R>
-__device__ __forceinline__ void statistics(const Raw<T, VEC> (*x)[K], int width, int lane, float inv_width, float eps, float* mean,
-                                           float* rstd, float (*buf)[8][32]) {
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    mean[r] = 0.f;
+  // Whether some of the piece is not the row's: the first one's and the last one's lanes.
+  __device__ __forceinline__ bool edge(int k) const { return SHIFT && (col(k) < 0 || col(k) + VEC > width); }
+  // `p`: the row's first element.  (Nothing is read behind the last row; before the first one lies nothing: its shift
+  // is 0.)
+  __device__ __forceinline__ void load(uint4* r, const T* p, int64_t row) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float f[VEC];
-      unpack<T, VEC>(x[r][k], f);
+      r[k] = make_uint4(0, 0, 0, 0);
+      if (row >= rows || !any(k)) continue;
+      if (SHIFT && row == rows - 1 && col(k) + VEC > width) {
+        T t[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) mean[r] += f[e];
-    }
-  }
-  row_sums<TPR, R>(mean, buf[0]);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    mean[r] *= inv_width;
-    rstd[r] = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (col_of<TPR, VEC>(lane, k) < width) {
-        float f[VEC];
-        unpack<T, VEC>(x[r][k], f);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) rstd[r] = fmaf(f[e] - mean[r], f[e] - mean[r], rstd[r]);
+        for (int e = 0; e < VEC; ++e) t[e] = has(k, e) ? p[col(k) + e] : from_f32<T>(0.f);
+        memcpy(&r[k], t, 16);
+      } else {
+        r[k] = *reinterpret_cast<const uint4*>(p + col(k));
       }
     }
   }
-  row_sums<TPR, R>(rstd, buf[1]);
+  // The values, 0 where they are not the row's.
+  __device__ __forceinline__ void values(const uint4* r, float* f) const {
 #pragma unroll
-  for (int r = 0; r < R; ++r) rstd[r] = rsqrtf(fmaf(rstd[r], inv_width, eps));
+    for (int k = 0; k < K; ++k) {
+      unpack<T>(r[k], f + k * VEC);
+      if (edge(k)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[k * VEC + e] = has(k, e) ? f[k * VEC + e] : 0.f;
+      }
+    }
+  }
+  // f - mean, 0 where the value is not the row's.
+  __device__ __forceinline__ void center(float* f, float mean) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float m = any(k) ? mean : 0.f;
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) fadd2(f[k * VEC + e], f[k * VEC + e + 1], f[k * VEC + e], f[k * VEC + e + 1], -m, -m);
+      if (edge(k)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[k * VEC + e] = has(k, e) ? f[k * VEC + e] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* p, const float* f) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!any(k)) continue;
+      if (edge(k)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (has(k, e)) p[col(k) + e] = from_f32<T>(f[k * VEC + e]);
+      } else {
+        *reinterpret_cast<uint4*>(p + col(k)) = pack<T>(f + k * VEC);
+      }
+    }
+  }
+  __device__ __forceinline__ void affine(const void* a, int dtype, float otherwise, float* w) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = a && has(i / VEC, i % VEC) ? affine_at(a, dtype, col(i / VEC) + i % VEC) : otherwise;
+  }
+};
+
+// The rows of a block: of class `first` modulo `step`, from the block's place among those of its class.
+struct BlockRows {
+  int64_t first, step, stride;   // stride: rows of the class between two turns of the block
+  int shift;
+};
+template <bool SHIFT>
+__device__ __forceinline__ BlockRows block_rows(const LayerNormArgs& a, int vec, int per_turn) {
+  if (!SHIFT) return {(int64_t)blockIdx.x * per_turn, 1, (int64_t)gridDim.x * per_turn, 0};
+  // (the grid is a multiple of the classes)
+  const int cls = blockIdx.x % a.classes, place = blockIdx.x / a.classes;
+  return {cls + (int64_t)place * per_turn * a.classes, a.classes, (int64_t)(gridDim.x / a.classes) * per_turn * a.classes,
+          (int)((int64_t)cls * a.width % vec)};
 }
 
-template <typename T, int VEC, int TPR, int K, int R>
+template <int E>
+__device__ __forceinline__ float sum_of(const float* f) {
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) fadd2(s0, s1, s0, s1, f[e], f[e + 1]);
+  return s0 + s1;
+}
+template <int E>
+__device__ __forceinline__ float dot_of(const float* f, const float* g) {
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) ffma2(s0, s1, f[e], f[e + 1], g[e], g[e + 1], s0, s1);
+  return s0 + s1;
+}
+
+template <typename T, int TPR, int K, int R, bool SHIFT>
 __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_fwd_kernel(LayerNormArgs a) {
   constexpr int kGroups = kBlock<TPR> / TPR;
-  __shared__ float buf[2][8][32];
-  const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  using P = RowPieces<T, TPR, K, SHIFT>;
+  constexpr int E = P::E;
+  __shared__ float buf[2][R][32];
+  const int grp = threadIdx.x / TPR;
+  const BlockRows rows = block_rows<SHIFT>(a, kVec<T>, kGroups * R);
+  const P p{(int)(threadIdx.x % TPR), a.width, rows.shift, a.rows};
   const float inv_width = 1.f / (float)a.width;
   after_previous();
-  float w[K * VEC], b[K * VEC];
-#pragma unroll
-  for (int i = 0; i < K * VEC; ++i) {
-    const int c = col_of<TPR, VEC>(lane, i / VEC) + i % VEC;
-    w[i] = a.weight && c < a.width ? affine_at(a.weight, a.affine_dtype, c) : 1.f;
-    b[i] = a.bias && c < a.width ? affine_at(a.bias, a.affine_dtype, c) : 0.f;
-  }
-  for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < a.rows; base += (int64_t)gridDim.x * kGroups * R) {
-    Raw<T, VEC> x[R][K];
+  float w[E], b[E];
+  p.affine(a.weight, a.affine_dtype, 1.f, w);
+  p.affine(a.bias, a.affine_dtype, 0.f, b);
+  uint4 raw[R][K];
+  auto load = [&](int64_t base) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + grp;
-      load_row<T, VEC, K>(x[r], reinterpret_cast<const T*>(a.x) + row * a.ld_x, row < a.rows, a.width, lane, TPR);
+      const int64_t row = base + (r * kGroups + grp) * rows.step;
+      p.load(raw[r], reinterpret_cast<const T*>(a.x) + row * a.ld_x, row);
     }
-    float mean[R], rstd[R];
-    statistics<T, VEC, TPR, K, R>(x, a.width, lane, inv_width, a.eps, mean, rstd, buf);
+  };
+  if (rows.first < a.rows) load(rows.first);
+  for (int64_t base = rows.first; base < a.rows; base += rows.stride) {
+    float f[R][E], mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + grp;
-      T* y = reinterpret_cast<T*>(a.y) + row * a.width;
+      p.values(raw[r], f[r]);
+      mean[r] = sum_of<E>(f[r]);
+    }
+    if (base + rows.stride < a.rows) load(base + rows.stride);   // on their way meanwhile
+    row_sums<TPR, R>(mean, buf[0]);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float f[VEC];
-        unpack<T, VEC>(x[r][k], f);
+    for (int r = 0; r < R; ++r) {
+      p.center(f[r], mean[r] * inv_width);
+      rstd[r] = dot_of<E>(f[r], f[r]);
+    }
+    row_sums<TPR, R>(rstd, buf[1]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = fmaf((f[e] - mean[r]) * rstd[r], w[k * VEC + e], b[k * VEC + e]);
-        const int c = col_of<TPR, VEC>(lane, k);
-        if (row < a.rows && c < a.width) *reinterpret_cast<Raw<T, VEC>*>(y + c) = pack<T, VEC>(f);
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + (r * kGroups + grp) * rows.step;
+      const float s = rsqrtf(fmaf(rstd[r], inv_width, a.eps));
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        fmul2(f[r][e], f[r][e + 1], f[r][e], f[r][e + 1], s, s);
+        ffma2(f[r][e], f[r][e + 1], f[r][e], f[r][e + 1], w[e], w[e + 1], b[e], b[e + 1]);
       }
+      if (row < a.rows) p.store(reinterpret_cast<T*>(a.y) + row * a.width, f[r]);
     }
   }
 }
 
-template <typename T, int VEC, int TPR, int K, int R>
+template <typename T, int TPR, int K, int R, bool SHIFT>
 __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_bwd_kernel(LayerNormArgs a) {
-  constexpr int kGroups = kBlock<TPR> / TPR, E = K * VEC;
-  __shared__ float buf[3][8][32];
-  const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  constexpr int kGroups = kBlock<TPR> / TPR;
+  using P = RowPieces<T, TPR, K, SHIFT>;
+  constexpr int E = P::E, VEC = P::VEC;
+  __shared__ float buf[2][2 * R][32];
+  const int grp = threadIdx.x / TPR;
+  const BlockRows rows = block_rows<SHIFT>(a, VEC, kGroups * R);
+  const P p{(int)(threadIdx.x % TPR), a.width, rows.shift, a.rows};
   const float inv_width = 1.f / (float)a.width;
   after_previous();
   float w[E], dw[E], db[E];
+  p.affine(a.weight, a.affine_dtype, 1.f, w);
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int c = col_of<TPR, VEC>(lane, i / VEC) + i % VEC;
-    w[i] = a.weight && c < a.width ? affine_at(a.weight, a.affine_dtype, c) : 1.f;
-    dw[i] = db[i] = 0.f;
-  }
-  for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < a.rows; base += (int64_t)gridDim.x * kGroups * R) {
-    Raw<T, VEC> x[R][K], dy[R][K];
+  for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.f;
+  uint4 raw_x[R][K], raw_dy[R][K];
+  auto load = [&](int64_t base) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + grp;
-      load_row<T, VEC, K>(x[r], reinterpret_cast<const T*>(a.x) + row * a.ld_x, row < a.rows, a.width, lane, TPR);
-      load_row<T, VEC, K>(dy[r], reinterpret_cast<const T*>(a.dy) + row * a.ld_dy, row < a.rows, a.width, lane, TPR);
+      const int64_t row = base + (r * kGroups + grp) * rows.step;
+      p.load(raw_x[r], reinterpret_cast<const T*>(a.x) + row * a.ld_x, row);
+      p.load(raw_dy[r], reinterpret_cast<const T*>(a.dy) + row * a.ld_dy, row);
     }
-    float mean[R], rstd[R], s[2 * R];
-    statistics<T, VEC, TPR, K, R>(x, a.width, lane, inv_width, a.eps, mean, rstd, buf);
-    // (elements behind the row, and rows behind the last, have dy = 0)
+  };
+  if (rows.first < a.rows) load(rows.first);
+  for (int64_t base = rows.first; base < a.rows; base += rows.stride) {
+    float f[R][E], d[R][E], s[2 * R], t[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s[2 * r] = s[2 * r + 1] = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float f[VEC], d[VEC];
-        unpack<T, VEC>(x[r][k], f);
-        unpack<T, VEC>(dy[r][k], d);
-        if (base + r * kGroups + grp < a.rows && col_of<TPR, VEC>(lane, k) < a.width) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float xh = (f[e] - mean[r]) * rstd[r], g = d[e] * w[k * VEC + e];
-            s[2 * r] += g;
-            s[2 * r + 1] = fmaf(g, xh, s[2 * r + 1]);
-            dw[k * VEC + e] = fmaf(d[e], xh, dw[k * VEC + e]);
-            db[k * VEC + e] += d[e];
-          }
-        }
-      }
+      p.values(raw_x[r], f[r]);
+      p.values(raw_dy[r], d[r]);     // (0 behind the last row)
+      s[2 * r] = sum_of<E>(f[r]);
+      s[2 * r + 1] = dot_of<E>(d[r], w);
     }
-    if (a.dx == nullptr) continue;
-    row_sums<TPR, 2 * R>(s, buf[2]);
+    if (base + rows.stride < a.rows) load(base + rows.stride);   // on their way meanwhile
+    row_sums<TPR, 2 * R>(s, buf[0]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * kGroups + grp;
-      const float m1 = s[2 * r] * inv_width, m2 = s[2 * r + 1] * inv_width;
-      T* dx = reinterpret_cast<T*>(a.dx) + row * a.width;
+      p.center(f[r], s[2 * r] * inv_width);
+      float t0 = 0.f, t1 = 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float f[VEC], d[VEC];
-        unpack<T, VEC>(x[r][k], f);
-        unpack<T, VEC>(dy[r][k], d);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float xh = (f[e] - mean[r]) * rstd[r];
-          f[e] = rstd[r] * (fmaf(d[e], w[k * VEC + e], -m1) - xh * m2);
-        }
-        const int c = col_of<TPR, VEC>(lane, k);
-        if (row < a.rows && c < a.width) *reinterpret_cast<Raw<T, VEC>*>(dx + c) = pack<T, VEC>(f);
+      for (int e = 0; e < E; e += 2) {
+        float g0, g1;
+        fmul2(g0, g1, d[r][e], d[r][e + 1], w[e], w[e + 1]);
+        ffma2(t0, t1, g0, g1, f[r][e], f[r][e + 1], t0, t1);
       }
+      t[2 * r] = dot_of<E>(f[r], f[r]);
+      t[2 * r + 1] = t0 + t1;
+    }
+    row_sums<TPR, 2 * R>(t, buf[1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + (r * kGroups + grp) * rows.step;
+      const float rstd = rsqrtf(fmaf(t[2 * r], inv_width, a.eps)), m1 = s[2 * r + 1] * inv_width, m2 = t[2 * r + 1] * rstd * inv_width;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        float &x0 = f[r][e], &x1 = f[r][e + 1], &d0 = d[r][e], &d1 = d[r][e + 1];
+        fmul2(x0, x1, x0, x1, rstd, rstd);
+        ffma2(dw[e], dw[e + 1], d0, d1, x0, x1, dw[e], dw[e + 1]);
+        fadd2(db[e], db[e + 1], db[e], db[e + 1], d0, d1);
+        ffma2(d0, d1, d0, d1, w[e], w[e + 1], -m1, -m1);
+        ffma2(d0, d1, x0, x1, -m2, -m2, d0, d1);
+        fmul2(d0, d1, d0, d1, rstd, rstd);
+      }
+      if (a.dx && row < a.rows) p.store(reinterpret_cast<T*>(a.dx) + row * a.width, d[r]);
     }
   }
   if (a.partials == nullptr) return;
   float* out = a.partials + (int64_t)blockIdx.x * 2 * a.width;
   if constexpr (TPR > 32) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int c = col_of<TPR, VEC>(lane, i / VEC) + i % VEC;
-      if (c < a.width) {
+    for (int i = 0; i < E; ++i)
+      if (p.has(i / VEC, i % VEC)) {
+        const int c = p.col(i / VEC) + i % VEC;
         out[c] = dw[i];
         out[a.width + c] = db[i];
       }
-    }
   } else {
     // rows of one warp, then the eight warps
     __shared__ float sum[8][2][TPR * E];
@@ -261,8 +330,8 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_bwd_kernel(LayerNormAr
         dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], m);
         db[i] += __shfl_xor_sync(0xffffffffu, db[i], m);
       }
-      const int c = col_of<TPR, VEC>(lane, i / VEC) + i % VEC;
-      if ((threadIdx.x & 31) < TPR) {
+      if ((threadIdx.x & 31) < TPR && p.has(i / VEC, i % VEC)) {
+        const int c = p.col(i / VEC) + i % VEC;
         sum[threadIdx.x >> 5][0][c] = dw[i];
         sum[threadIdx.x >> 5][1][c] = db[i];
       }
@@ -391,28 +460,38 @@ cudaError_t sum_blocks(const LayerNormArgs& a, int blocks, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ dispatch
-// Threads a row and elements a thread, by width.
+// Threads a row and elements a thread, by the elements of its pieces.
 struct RowShape {
   int tpr, e;
 };
 constexpr RowShape row_shape(int width) {
-  return width <= 64 ? RowShape{8, 8}
-         : width <= 128 ? RowShape{16, 8}
-         : width <= 256 ? RowShape{32, 8}
+  return width <= 64 ? RowShape{4, 16}
+         : width <= 128 ? RowShape{8, 16}
+         : width <= 256 ? RowShape{16, 16}
          : width <= 512 ? RowShape{32, 16}
          : width <= 1024 ? RowShape{128, 8}
          : width <= 2048 ? RowShape{128, 16}
          : width <= 4096 ? RowShape{256, 16}
                          : RowShape{512, 16};
 }
+// Classes of rows that begin at the same place of a 16-byte piece, and the elements of a row's pieces.
+int row_classes(int width, int vec) {
+  int c = vec;
+  while (c > 1 && width % 2 == 0) {
+    width /= 2;
+    c /= 2;
+  }
+  return c;
+}
+int pieces_width(int width, int vec) { return row_classes(width, vec) > 1 ? width + vec - 1 : width; }
 // Blocks of the backward at most: eight a multiprocessor (three of whole rows, whose partial sums are wide).
 constexpr int most_blocks(int tpr) { return 148 * (tpr > 32 ? 3 : 8); }
-constexpr int kFwdRows = 4, kBwdRows = 2;   // rows a group of threads has in flight
 
-int64_t bwd_blocks(int64_t rows, int width) {
-  const int tpr = row_shape(width).tpr;
-  const int64_t per = (int64_t)(tpr > 32 ? 1 : 256 / tpr) * kBwdRows, b = (rows + per - 1) / per;
-  return b < most_blocks(tpr) ? b : most_blocks(tpr);
+int64_t bwd_blocks(int64_t rows, int width, int vec) {
+  const int tpr = row_shape(pieces_width(width, vec)).tpr, classes = row_classes(width, vec);
+  const int64_t per = tpr > 32 ? 1 : 256 / tpr, b = (rows + per - 1) / per;
+  const int64_t most = b < most_blocks(tpr) ? b : most_blocks(tpr);
+  return (most + classes - 1) / classes * classes;
 }
 
 template <auto Kernel>
@@ -426,36 +505,41 @@ int blocks_per_sm(int threads) {
   return b;
 }
 
-template <typename T, int VEC, int TPR, int E, bool BWD>
+template <typename T, int TPR, int E, bool SHIFT, bool BWD>
 cudaError_t launch_row(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
-  constexpr int kThreads = kBlock<TPR>, R = BWD ? kBwdRows : (E > 8 ? kFwdRows / 2 : kFwdRows);
+  // rows that a group of threads works on at a time; in the backward two where it is a block of 128, which waits
+  // for all of its threads twice a turn (more threads leave no registers for it)
+  constexpr int kThreads = kBlock<TPR>, R = BWD && TPR != 128 ? 1 : 2, K = E / kVec<T>;
   constexpr auto kern = [] {
-    if constexpr (BWD) return &layer_norm_bwd_kernel<T, VEC, TPR, E / VEC, R>;
-    else return &layer_norm_fwd_kernel<T, VEC, TPR, E / VEC, R>;
+    if constexpr (BWD) return &layer_norm_bwd_kernel<T, TPR, K, R, SHIFT>;
+    else return &layer_norm_fwd_kernel<T, TPR, K, R, SHIFT>;
   }();
   const int64_t per = (int64_t)(kThreads / TPR) * R, need = (a.rows + per - 1) / per;
   int64_t most = (int64_t)sm_count() * blocks_per_sm<kern>(kThreads);
   if (BWD && most > most_blocks(TPR)) most = most_blocks(TPR);
-  *blocks = (int)(need < most ? need : most);
+  if (need < most) most = need;
+  *blocks = (int)(SHIFT ? (most + a.classes - 1) / a.classes * a.classes : most);
   return launch_early(kern, dim3((unsigned)*blocks), kThreads, 0, s, a);
 }
 
-template <typename T, int VEC, bool BWD>
+template <typename T, bool SHIFT, bool BWD>
 cudaError_t launch_width(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
-  const RowShape r = row_shape(a.width);
+  const RowShape r = row_shape(pieces_width(a.width, kVec<T>));
   switch (r.tpr) {
-    case 8: return launch_row<T, VEC, 8, 8, BWD>(a, s, blocks);
-    case 16: return launch_row<T, VEC, 16, 8, BWD>(a, s, blocks);
-    case 32: return r.e == 8 ? launch_row<T, VEC, 32, 8, BWD>(a, s, blocks) : launch_row<T, VEC, 32, 16, BWD>(a, s, blocks);
-    case 128: return r.e == 8 ? launch_row<T, VEC, 128, 8, BWD>(a, s, blocks) : launch_row<T, VEC, 128, 16, BWD>(a, s, blocks);
-    case 256: return launch_row<T, VEC, 256, 16, BWD>(a, s, blocks);
-    default: return launch_row<T, VEC, 512, 16, BWD>(a, s, blocks);
+    case 4: return launch_row<T, 4, 16, SHIFT, BWD>(a, s, blocks);
+    case 8: return launch_row<T, 8, 16, SHIFT, BWD>(a, s, blocks);
+    case 16: return launch_row<T, 16, 16, SHIFT, BWD>(a, s, blocks);
+    case 32: return launch_row<T, 32, 16, SHIFT, BWD>(a, s, blocks);
+    case 128: return r.e == 8 ? launch_row<T, 128, 8, SHIFT, BWD>(a, s, blocks) : launch_row<T, 128, 16, SHIFT, BWD>(a, s, blocks);
+    case 256: return launch_row<T, 256, 16, SHIFT, BWD>(a, s, blocks);
+    default: return launch_row<T, 512, 16, SHIFT, BWD>(a, s, blocks);
   }
 }
 
 template <typename T, bool BWD>
-cudaError_t launch_type(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
-  if (a.width > kMaxRow) {
+cudaError_t launch_type(LayerNormArgs a, cudaStream_t s, int* blocks) {
+  a.classes = row_classes(a.width, kVec<T>);
+  if (pieces_width(a.width, kVec<T>) > kMaxRow) {
     const unsigned grid = (unsigned)(a.rows < 4 * sm_count() ? a.rows : 4 * sm_count());
     float* stats = nullptr;
     *blocks = (int)((a.rows + kLongRows - 1) / kLongRows);
@@ -464,11 +548,8 @@ cudaError_t launch_type(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
     if (e != cudaSuccess || !stats) return e;
     return launch_early(layer_norm_columns_kernel<T>, dim3((unsigned)((a.width + 255) / 256), (unsigned)*blocks), 256, 0, s, a, (const float*)stats);
   }
-  constexpr int kVec = 16 / sizeof(T);
-  auto whole = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  const bool vec = a.width % kVec == 0 && whole(a.x) && whole(a.y) && whole(a.dx) && whole(a.dy) &&
-                   (a.rows == 1 || (a.ld_x % kVec == 0 && (!BWD || a.ld_dy % kVec == 0)));
-  return vec ? launch_width<T, kVec, BWD>(a, s, blocks) : launch_width<T, 1, BWD>(a, s, blocks);
+  if (a.classes == 1) return launch_width<T, false, BWD>(a, s, blocks);
+  return launch_width<T, true, BWD>(a, s, blocks);
 }
 
 template <bool BWD>
@@ -482,9 +563,15 @@ cudaError_t launch_any(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
 
 }  // namespace
 
-int64_t layer_norm_workspace_floats(int64_t rows, int width, int) {
-  if (width > kMaxRow) return (rows + kLongRows - 1) / kLongRows * 2 * width + 2 * rows;
-  return bwd_blocks(rows, width) * 2 * width;
+bool layer_norm_rows_fit(int64_t ld, int width, int dtype) {
+  const int vec = dtype == TRIFAST_F32 ? 4 : 8;
+  return (ld - width) % vec == 0;
+}
+
+int64_t layer_norm_workspace_floats(int64_t rows, int width, int dtype) {
+  const int vec = dtype == TRIFAST_F32 ? 4 : 8;
+  if (pieces_width(width, vec) > kMaxRow) return (rows + kLongRows - 1) / kLongRows * 2 * width + 2 * rows;
+  return bwd_blocks(rows, width, vec) * 2 * width;
 }
 
 cudaError_t layer_norm_forward(const LayerNormArgs& a, cudaStream_t s) {

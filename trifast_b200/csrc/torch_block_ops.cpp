@@ -42,6 +42,9 @@ struct Rows {
   Tensor t;
   int64_t rows, ld;
 };
+Rows dense_rows(const Tensor& t) {
+  return {t.clone(at::MemoryFormat::Contiguous), t.numel() / t.size(-1), t.size(-1)};
+}
 Rows as_rows(const Tensor& t) {
   const int64_t width = t.size(-1), rows = t.numel() / width;
   int64_t ld = width, next = -1;   // next: what the stride of the next dimension outwards must be
@@ -54,8 +57,12 @@ Rows as_rows(const Tensor& t) {
       ok = t.stride(d) == next;
     next = t.stride(d) * t.size(d);
   }
-  if (ok && ld >= width) return {t, rows, ld};
-  return {t.clone(at::MemoryFormat::Contiguous), rows, width};
+  return ok && ld >= width ? Rows{t, rows, ld} : dense_rows(t);
+}
+// The same for layer norm, whose rows lie a multiple of 16 bytes beyond their width.
+Rows as_norm_rows(const Tensor& t) {
+  const Rows r = as_rows(t);
+  return (r.ld - t.size(-1)) * t.element_size() % 16 == 0 ? r : dense_rows(t);
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
@@ -110,7 +117,7 @@ Tensor layer_norm_cuda(const Tensor& x, const optional<Tensor>& weight_, const o
   raise_if_device_gave_up(x.device().index(), stream);
   Tensor y = at::empty(x.sizes(), x.options());
   if (x.numel() == 0) return y;
-  const Rows r = as_rows(x);
+  const Rows r = as_norm_rows(x);
   n.rows = r.rows;
   n.ld_x = r.ld;
   if (weight.defined()) weight = dense(weight);
@@ -142,8 +149,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_grads_cuda(const Tensor& dy, const
   if (want_bias) db = at::empty({n.width}, weight.options());
   Rows rx{x, 0, n.width}, rdy{dy, 0, n.width};
   if (x.numel() != 0) {
-    rx = as_rows(x);
-    rdy = as_rows(dy);
+    rx = as_norm_rows(x);
+    rdy = as_norm_rows(dy);
   }
   n.rows = rx.rows;
   n.ld_x = rx.ld;
