@@ -297,5 +297,5 @@ def test_workspace_of_the_feed_forward_does_not_grow_with_the_rows():
     lib = _lib.load()
     for dtype in (0, 1):
         size = [lib.trifast_feed_forward_backward_workspace_bytes(byref(_lib.FeedForward(r, 128, 128, 128, 512, 128, dtype)))
-                for r in (1 << 18, 1 << 20, 1 << 30)]
-        assert all(0 < s < 160 << 20 for s in size)
+                for r in (1 << 20, 1 << 24, 1 << 30)]
+        assert all(0 < s < 320 << 20 for s in size)

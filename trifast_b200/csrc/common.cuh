@@ -128,19 +128,27 @@ __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.
 // Launches a kernel that calls after_previous().  Against plain launches, h = 4, d = 32, calls back to
 // back: forward and backward (six kernels) at n = 256 154.8 -> 143.8 us, n = 384 428 -> 415, n = 512 (15 %
 // padding) 823 -> 813; forward alone at n = 733 703 -> 699 us.
+// cluster: CTAs to a cluster.
 template <typename... P, typename... A>
-cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A&&... args) {
+cudaError_t launch_clusters(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, int cluster, A&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A&&... args) {
+  return launch_clusters(kernel, grid, threads, smem, s, 1, static_cast<A&&>(args)...);
 }
 
 // SMs of the current device.

@@ -6,7 +6,10 @@
 // on the tensor cores, as one kernel with four epilogues (Mode in ff_gemm.cuh).
 //
 // A tile has 128 rows and up to 256 fp32 columns in TMEM, twice, so that the epilogue of one tile runs
-// under the MMAs of the next.  Operands come in blocks of 64 along the contraction, through a ring of
+// under the MMAs of the next.  (kHidden has 128 units a tile: a and b once, 256 columns, dH twice, so that the next dH
+// runs under the epilogue: with 64 units, all of them twice, X and dY came from L2 twice as often, which bounds this
+// kernel: 72 us for 8192 rows, width 512, hidden 2048.)  Where there is more than one row tile, two CTAs share an MMA (CG = 2): each has its 128
+// rows of A and of the result, and half of B's tile, which the tensor cores of both read.  Operands come in blocks of 64 along the contraction, through a ring of
 // stages that TMA fills (128-byte swizzle).  Both majors are read as they lie: where the contraction
 // runs along a matrix's rows the tile is an MN-major operand of 64-element columns.  CTAs are
 // persistent, one per SM, the tiles of one row block next to one another.
@@ -36,17 +39,17 @@ constexpr int kThreads = 320;
 constexpr int kSmemLimit = 232448;
 
 // Columns per B matrix (NT), accumulator columns, stages and staging of results by mode.
-template <int MODE, int NT>
+template <int MODE, int NT, int CG>
 struct Cfg {
-  static constexpr int kAccCols = MODE == kGate ? 2 * NT : MODE == kHidden ? 3 * NT : NT;
-  static constexpr int kBRows = MODE == kGate || MODE == kHidden ? 2 * NT : NT;   // largest of a stage
-  static constexpr int kStageBytes = kTileA + kBRows * kBK * 2;
+  static constexpr int kAccCols = MODE == kGate || MODE == kHidden ? 2 * NT : NT;
+  static constexpr int kBRows = MODE == kGate || MODE == kHidden ? 2 * NT : NT;   // largest of a stage, in all
+  static constexpr int kStageBytes = kTileA + kBRows / CG * kBK * 2;
   // result tiles of 128 rows x 64 columns
   static constexpr int kOutTiles = MODE == kGate ? NT / 64 : MODE == kHidden ? 3 : MODE == kLinear ? 2 : 0;
   static constexpr int kStages = (kSmemLimit - 2048 - kOutTiles * kTileA) / kStageBytes;
   static constexpr int kBufCols = kAccCols > 128 ? 256 : 128;    // TMEM columns between the two buffers
   static constexpr int smem_bytes() { return 1024 + 1024 + kStages * kStageBytes + kOutTiles * kTileA; }
-  static_assert(kAccCols <= 256 && kStages >= 4 && smem_bytes() <= kSmemLimit, "tile configuration");
+  static_assert(kAccCols <= 256 && kStages >= 3 && smem_bytes() <= kSmemLimit, "tile configuration");
 };
 
 struct Params {
@@ -85,8 +88,8 @@ struct TileAt {
   int job, split;
 };
 
-template <int MODE, int NT>
-__device__ __forceinline__ TileAt tile_at(const Params& p, int t) {
+template <int MODE, int NT, int CG>
+__device__ __forceinline__ TileAt tile_at(const Params& p, int t, int rank) {
   TileAt r;
   r.job = 0;
   r.split = 0;
@@ -101,20 +104,22 @@ __device__ __forceinline__ TileAt tile_at(const Params& p, int t) {
       }
   }
   const int nt = p.n_tiles[r.job];
-  r.m0 = (t / nt) * 128;
+  r.m0 = (t / nt) * 128 * CG + rank * 128;
   r.n0 = (t % nt) * NT;
   return r;
 }
 
 // T: type of the operands; PARTS: planes of each (1, or 3 for fp32); OUT: type of kLinear's result.
-template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN>
+template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN, int CG>
 __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<MODE, NT>;
+  using C = Cfg<MODE, NT, CG>;
   constexpr int S = C::kStages;
   constexpr int FULL = 0, EMPTY = S, ACC_FULL = 2 * S, ACC_EMPTY = 2 * S + 2, NBARS = 2 * S + 4;
   static_assert(NBARS * 8 <= 240, "barrier area");
   constexpr int kPairs = PARTS == 1 ? 1 : 6;
   constexpr bool kAMn = MODE == kWeight;
+  constexpr bool kOneAB = MODE == kHidden && PARTS == 1;   // a and b have one place in TMEM, dH two
+  constexpr int kDhCol = 256;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -123,12 +128,16 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + 256);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + 260);
   auto bar = [&](int i) -> uint32_t { return base + 8u * i; };
+  const int rank = CG == 2 ? (int)cluster_rank() : 0;
+  // (the pair's first CTA counts what arrives, issues the MMAs and is told when results have been read)
+  auto first_bar = [&](int i) -> uint32_t { return CG == 2 ? in_cta(bar(i), 0) : bar(i); };
   auto a_tile = [&](int s) -> uint32_t { return base + 1024 + s * C::kStageBytes; };
   auto b_tile = [&](int s) -> uint32_t { return a_tile(s) + kTileA; };
   constexpr uint32_t out_off = 1024 + S * C::kStageBytes;
 
   after_previous();
-  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+  const bool given_up = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
+  if (CG == 1 && given_up) return;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -138,19 +147,28 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ACC_FULL + i), 1);
-      mbar_init(bar(ACC_EMPTY + i), 8);
+      mbar_init(bar(ACC_EMPTY + i), 8 * CG);
     }
     *abort_flag = 0;
+    if (CG == 2) *reinterpret_cast<volatile uint32_t*>(gbase + 264) = given_up;
     mbar_fence_init();
   }
   if (warp == 9) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
-    tmem_relinquish();
+    if (CG == 2) {
+      tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // both CTAs of a pair go on, or neither
+  bool go = true;
+  if (CG == 2) go = (load_cluster(in_cta(base + 264, 0)) | load_cluster(in_cta(base + 264, 1))) == 0;
 
   // blocks of the contraction of phase ph of a tile
   auto k_range = [&](const TileAt& t, int ph, int& lo, int& hi) {
@@ -164,12 +182,13 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
   };
   const int phases = MODE == kHidden ? 2 : MODE == kLinear ? p.phases : 1;
 
-  if (warp == 8) {
+  if (!go) {
+  } else if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
     int g = 0;
     bool ok = true;
-    for (int w = blockIdx.x; w < p.tiles && ok; w += gridDim.x) {
-      const TileAt t = tile_at<MODE, NT>(p, w);
+    for (int w = blockIdx.x / CG; w < p.tiles && ok; w += gridDim.x / CG) {
+      const TileAt t = tile_at<MODE, NT, CG>(p, w, rank);
       for (int ph = 0; ph < phases && ok; ++ph) {
         int lo, hi;
         k_range(t, ph, lo, hi);
@@ -182,35 +201,54 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (elect_one()) {
-              const uint32_t f = bar(FULL + s);
+              const uint32_t f = first_bar(FULL + s);
               const int kc = kb * kBK;
-              if constexpr (MODE == kHidden) {
-                mbar_arrive_expect_tx(f, kTileA + (ph == 0 ? 2 : 1) * NT * kBK * 2);
-                tma_load_3d(a_tile(s), ma, f, kc, t.m0, pa);
-                if (ph == 0) {
-                  tma_load_3d(b_tile(s), &p.b[0], f, kc, t.n0, pb);
-                  tma_load_3d(b_tile(s) + NT * kBK * 2, &p.b[1], f, kc, t.n0, pb);
+              // (the first CTA's arrival, with the bytes of both)
+              auto expect = [&](int bytes) {
+                if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), CG * bytes);
+              };
+              auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+                if (CG == 2)
+                  tma_load_3d_pair(dst, map, f, c0, c1, c2);
+                else
+                  tma_load_3d(dst, map, f, c0, c1, c2);
+              };
+              // Wg and Wu: one each of the pair
+              auto load_gate_up = [&] {
+                if (CG == 2) {
+                  load(b_tile(s), &p.b[rank], kc, t.n0, pb);
                 } else {
-                  tma_load_3d(b_tile(s), &p.b[2], f, t.n0, kc, pb);
+                  load(b_tile(s), &p.b[0], kc, t.n0, pb);
+                  load(b_tile(s) + NT * kBK * 2, &p.b[1], kc, t.n0, pb);
+                }
+              };
+              if constexpr (MODE == kHidden) {
+                expect(kTileA + (ph == 0 ? 1 : 2) * NT / CG * kBK * 2);
+                load(a_tile(s), ma, kc, t.m0, pa);
+                if (ph == 0) {
+#pragma unroll
+                  for (int i = 0; i < NT / CG / 64; ++i) load(b_tile(s) + i * 8192, &p.b[2], t.n0 + rank * (NT / CG) + 64 * i, kc, pb);
+                } else {
+                  load_gate_up();
                 }
               } else {
-                mbar_arrive_expect_tx(f, C::kStageBytes);
+                expect(C::kStageBytes);
                 if constexpr (kAMn) {
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) tma_load_3d(a_tile(s) + i * 8192, ma, f, t.m0 + 64 * i, kc, pa);
+                  for (int i = 0; i < 2; ++i) load(a_tile(s) + i * 8192, ma, t.m0 + 64 * i, kc, pa);
                 } else {
-                  tma_load_3d(a_tile(s), ma, f, kc, t.m0, pa);
+                  load(a_tile(s), ma, kc, t.m0, pa);
                 }
                 if constexpr (MODE == kGate) {
-                  tma_load_3d(b_tile(s), &p.b[0], f, kc, t.n0, pb);
-                  tma_load_3d(b_tile(s) + NT * kBK * 2, &p.b[1], f, kc, t.n0, pb);
+                  load_gate_up();
                 } else {
                   const CUtensorMap* mb = &p.b[MODE == kWeight ? t.job : ph];
+                  const int n0 = t.n0 + rank * (NT / CG);
                   if constexpr (B_MN) {
 #pragma unroll
-                    for (int i = 0; i < NT / 64; ++i) tma_load_3d(b_tile(s) + i * 8192, mb, f, t.n0 + 64 * i, kc, pb);
+                    for (int i = 0; i < NT / CG / 64; ++i) load(b_tile(s) + i * 8192, mb, n0 + 64 * i, kc, pb);
                   } else {
-                    tma_load_3d(b_tile(s), mb, f, kc, t.n0, pb);
+                    load(b_tile(s), mb, kc, n0, pb);
                   }
                 }
               }
@@ -220,25 +258,37 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         }
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 9 && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     int g = 0, it = 0;   // running stage, and running sum (a buffer of TMEM)
     bool ok = true;
     uint32_t acc = tmem_base;
-    auto open_sum = [&] {
-      acc = tmem_base + (it & 1) * C::kBufCols;
-      if (it >= 2) ok = mbar_wait(bar(ACC_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, abort_flag);
+    auto wait_read = [&](int sum) {   // until the epilogue has read this sum
+      const int e = ACC_EMPTY + (sum & 1), parity = (sum >> 1) & 1;
+      if (sum >= 0) ok = CG == 2 ? mbar_wait_cluster(bar(e), parity, abort_flag) : mbar_wait(bar(e), parity, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     };
+    auto open_sum = [&] {
+      acc = tmem_base + (it & 1) * C::kBufCols;
+      // (kHidden's dH goes where that of the sum before the last was, which has been read: a and b of the last sum
+      // waited for it)
+      if (!kOneAB) wait_read(it - 2);
+    };
+    auto commit = [&](int b) {
+      if (CG == 2)
+        umma_commit_pair(bar(b));
+      else
+        umma_commit(bar(b));
+    };
     auto close_sum = [&] {
-      if (elect_one()) umma_commit(bar(ACC_FULL + (it & 1)));
+      if (elect_one()) commit(ACC_FULL + (it & 1));
       __syncwarp();
       ++it;
     };
-    for (int w = blockIdx.x; w < p.tiles && ok; w += gridDim.x) {
-      const TileAt t = tile_at<MODE, NT>(p, w);
+    for (int w = blockIdx.x / CG; w < p.tiles && ok; w += gridDim.x / CG) {
+      const TileAt t = tile_at<MODE, NT, CG>(p, w, rank);
       open_sum();
       for (int ph = 0; ph < phases && ok; ++ph) {
         int lo, hi;
@@ -248,7 +298,11 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
           close_sum();
           open_sum();
         }
-        // (kLinear's two products add up in one accumulator; kHidden's second phase has its own)
+        if (kOneAB && ph == 1) {
+          wait_read(it - 1);
+          if (!ok) break;
+        }
+        // (kLinear's two products add up in one accumulator; kHidden's phases have their own)
         bool first = PARTS == 3 || MODE != kLinear || ph == 0;
         for (int i = 0; i < steps && ok; ++i, ++g) {
           if (PARTS == 3 && i > small && (i - small) % kSumStages == 0) {
@@ -263,18 +317,24 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const bool second = MODE == kHidden && ph == 1;
-            const bool bmn = second || B_MN;
-            const uint32_t idesc = second ? make_idesc(128, NT, kBf16, false, true)
-                                          : make_idesc(128, C::kBRows, kBf16, kAMn, B_MN);
-            const uint32_t d = acc + (second ? 2 * NT : 0);
+            const bool dh = MODE == kHidden && ph == 0;
+            const bool bmn = dh || B_MN;
+            const uint32_t idesc = dh ? make_idesc(128 * CG, NT, kBf16, false, true)
+                                      : make_idesc(128 * CG, C::kBRows, kBf16, kAMn, B_MN);
+            const uint32_t d = !kOneAB ? acc : dh ? tmem_base + kDhCol + (it & 1) * NT : tmem_base;
             const uint64_t ad = make_smem_desc(a_tile(s), kAMn ? 8192 : 16, 1024, kSwizzle128);
             const uint64_t bd = make_smem_desc(b_tile(s), bmn ? 8192 : 16, 1024, kSwizzle128);
             // 16 of the contraction: 32 bytes along a row, or 16 rows of an MN-major tile
             const uint32_t sa = kAMn ? 2048 >> 4 : 32 >> 4, sb = bmn ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk) umma_ss(d, ad + kk * sa, bd + kk * sb, idesc, (kk > 0 || !first) ? 1u : 0u);
-            umma_commit(bar(EMPTY + s));
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              const uint32_t add = (kk > 0 || !first) ? 1u : 0u;
+              if (CG == 2)
+                umma_ss_pair(d, ad + kk * sa, bd + kk * sb, idesc, add);
+              else
+                umma_ss(d, ad + kk * sa, bd + kk * sb, idesc, add);
+            }
+            commit(EMPTY + s);
           }
           __syncwarp();
           first = false;
@@ -283,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
       if (!ok) break;
       close_sum();
     }
-  } else {
+  } else if (warp < 8) {
     // ------------------------------------------------------------ epilogue
     const int grp = warp >> 2, wq = warp & 3, row = tid & 127;
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
@@ -309,14 +369,19 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
     auto release = [&] {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(ACC_EMPTY + (it & 1)));
+      if (lane == 0) {
+        if (CG == 2)
+          mbar_arrive_cluster(first_bar(ACC_EMPTY + (it & 1)));
+        else
+          mbar_arrive(bar(ACC_EMPTY + (it & 1)));
+      }
       ++it;
     };
     // PARTS = 3: this thread's columns of each matrix, added up over the sums
     constexpr int kCols = NT / 2, kSets = MODE == kGate ? 2 : MODE == kHidden ? 3 : 1;
     float total[PARTS == 3 ? kSets : 1][PARTS == 3 ? kCols : 1];
-    for (int w = blockIdx.x; w < p.tiles; w += gridDim.x) {
-      const TileAt t = tile_at<MODE, NT>(p, w);
+    for (int w = blockIdx.x / CG; w < p.tiles; w += gridDim.x / CG) {
+      const TileAt t = tile_at<MODE, NT, CG>(p, w, rank);
       bool none = false;   // an empty contraction: its sum is 0, and nothing wrote TMEM
       if constexpr (MODE == kWeight) {
         int lo, hi;
@@ -340,14 +405,14 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
             wait_sum();
             if (!ok) break;
             constexpr int kLast = kSets;
-            const int m0 = MODE == kHidden && ph == 1 ? 2 : 0, m1 = MODE == kHidden && ph == 0 ? 2 : kLast;
+            const int m0 = MODE == kHidden && ph == 0 ? 2 : 0, m1 = MODE == kHidden && ph == 1 ? 2 : kLast;
 #pragma unroll
             for (int m = 0; m < kSets; ++m) {
               if (m < m0 || m >= m1) continue;
 #pragma unroll
               for (int c = 0; c < kCols; c += 32) {
                 float v[32];
-                tmem_ld32(acc + m * NT + grp * kCols + c, reinterpret_cast<uint32_t*>(v));
+                tmem_ld32(acc + (m - m0) * NT + grp * kCols + c, reinterpret_cast<uint32_t*>(v));
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) total[m][c + e] += none ? 0.f : v[e];
@@ -405,54 +470,64 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
           }
           fence_async_smem();
           group_sync(bar_id, kBarThreads);
-          if (leader && col < p.n[0]) {
+          if (leader && col < p.n[0] && t.m0 < p.m[0]) {
             tma_store_3d(&p.out[0], base + out_off + tile * kTileA, col, t.m0, q);
             bulk_commit();
           }
         }
       } else if constexpr (MODE == kHidden) {
-        static_assert(MODE != kHidden || NT == 64, "result tiles are 64 columns");
-        float r[3][32];               // PARTS = 3; else packed
-        uint32_t packed[3][16];
-        {
-          float a[32], b[32], dh[32];
-          columns(0, 0, a);
-          columns(1, 0, b);
-          columns(2, 0, dh);
-          loaded(true);
-          if constexpr (PARTS == 1) {
-            grad_units<T, 32, true>(a, b, dh, packed[0], packed[1], packed[2]);
-          } else {
+        static_assert(MODE != kHidden || NT == (PARTS == 1 ? 128 : 64), "units of a tile");
+        // 64 units at a time, each group half of them
+#pragma unroll 1
+        for (int u0 = 0; u0 < NT; u0 += 64) {
+          float r[3][32];               // PARTS = 3; else packed
+          uint32_t packed[3][16];
+          {
+            float a[32], b[32], dh[32];
+            if constexpr (PARTS == 1) {
+              const uint32_t at = tmem_base + lane_base + u0 + grp * 32;
+              tmem_ld32(at, reinterpret_cast<uint32_t*>(a));
+              tmem_ld32(at + NT, reinterpret_cast<uint32_t*>(b));
+              tmem_ld32(at + kDhCol + (it & 1) * NT, reinterpret_cast<uint32_t*>(dh));
+              tmem_wait_ld();
+              if (u0 + 64 == NT) release();
+              grad_units<T, 32, true>(a, b, dh, packed[0], packed[1], packed[2]);
+            } else {
+              columns(0, 0, a);
+              columns(1, 0, b);
+              columns(2, 0, dh);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float s = sigmoid(a[e]), u = a[e] * s;
-              r[0][e] = dh[e] * b[e] * fmaf(u, 1.f - s, s);
-              r[1][e] = dh[e] * u;
-              r[2][e] = u * b[e];
+              for (int e = 0; e < 32; ++e) {
+                const float s = sigmoid(a[e]), u = a[e] * s;
+                r[0][e] = dh[e] * b[e] * fmaf(u, 1.f - s, s);
+                r[1][e] = dh[e] * u;
+                r[2][e] = u * b[e];
+              }
             }
           }
-        }
+          const int col = t.n0 + u0;
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-          if (leader) bulk_wait_read();
-          group_sync(bar_id, kBarThreads);
+          for (int q = 0; q < PARTS; ++q) {
+            if (leader) bulk_wait_read();
+            group_sync(bar_id, kBarThreads);
 #pragma unroll
-          for (int o = 0; o < 3; ++o)
+            for (int o = 0; o < 3; ++o)
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              if constexpr (PARTS == 3) {
+              for (int c = 0; c < 32; c += 8) {
+                if constexpr (PARTS == 3) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) packed[o][(c + e) >> 1] = take_part(r[o][c + e], r[o][c + e + 1]);
+                  for (int e = 0; e < 8; e += 2) packed[o][(c + e) >> 1] = take_part(r[o][c + e], r[o][c + e + 1]);
+                }
+                const uint32_t* u = packed[o] + c / 2;
+                *out_piece(o, (grp * 32 + c) >> 3) = make_uint4(u[0], u[1], u[2], u[3]);
               }
-              const uint32_t* u = packed[o] + c / 2;
-              *out_piece(o, (grp * 32 + c) >> 3) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          fence_async_smem();
-          group_sync(bar_id, kBarThreads);
-          if (leader) {
+            fence_async_smem();
+            group_sync(bar_id, kBarThreads);
+            if (leader && t.m0 < p.m[0] && col < p.n[0]) {
 #pragma unroll
-            for (int o = 0; o < 3; ++o) tma_store_3d(&p.out[o], base + out_off + o * kTileA, t.n0, t.m0, q);
-            bulk_commit();
+              for (int o = 0; o < 3; ++o) tma_store_3d(&p.out[o], base + out_off + o * kTileA, col, t.m0, q);
+              bulk_commit();
+            }
           }
         }
       } else if constexpr (MODE == kLinear) {
@@ -492,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
             if (p.y_tma) {
               fence_async_smem();
               group_sync(bar_id, kBarThreads);
-              if (leader && col < p.n[0]) {
+              if (leader && col < p.n[0] && t.m0 < p.m[0]) {
                 tma_store_3d(&p.out[0], base + out_off + grp * kTileA, col, t.m0, 0);
                 bulk_commit();
               }
@@ -562,17 +637,28 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
     if (tid == 0) set_status(p.status, kStatusTimeoutFeedForward);
     __syncthreads();
   }
+  // (neither CTA of a pair goes before the other's last access to it)
+  if (CG == 2) cluster_sync();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if (CG == 2)
+      tmem_dealloc_pair(tmem_base, 512);
+    else
+      tmem_dealloc(tmem_base, 512);
   }
 }
 
 int64_t tiles_of(int64_t x, int tile) { return (x + tile - 1) / tile; }
 
-template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN>
-cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
-  using C = Cfg<MODE, NT>;
+bool weight_pairs(bool f32, std::initializer_list<int64_t> m) {
+  for (int64_t c : m)
+    if (f32 || c <= 128) return false;
+  return true;
+}
+
+template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN, int CG>
+cudaError_t launch_group(const GemmArgs& g, cudaStream_t stream) {
+  using C = Cfg<MODE, NT, CG>;
   Params p = {};
   bool ok = true;
   int64_t tiles = 0;
@@ -581,7 +667,7 @@ cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
       p.m[j] = g.a[j].cols;
       p.n[j] = g.b[j].cols;
       p.k[j] = g.a[j].rows;
-      p.m_tiles[j] = (int)tiles_of(p.m[j], 128);
+      p.m_tiles[j] = (int)tiles_of(p.m[j], 128 * CG);
       p.n_tiles[j] = (int)tiles_of(p.n[j], NT);
       tiles += (int64_t)p.m_tiles[j] * p.n_tiles[j] * g.splits;
       ok = ok && map_of(&p.a[j], g.bf16, g.a[j], 64, kBK) && map_of(&p.b[j], g.bf16, g.b[j], 64, kBK);
@@ -590,7 +676,7 @@ cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
     p.phases = MODE == kHidden ? 2 : MODE == kLinear ? g.products : 1;
     p.m[0] = g.a[0].rows;
     p.n[0] = MODE == kLinear && B_MN ? g.b[0].cols : g.b[0].rows;
-    p.m_tiles[0] = (int)tiles_of(p.m[0], 128);
+    p.m_tiles[0] = (int)tiles_of(p.m[0], 128 * CG);
     p.n_tiles[0] = (int)tiles_of(p.n[0], NT);
     tiles = (int64_t)p.m_tiles[0] * p.n_tiles[0];
     for (int i = 0; i < p.phases; ++i) {
@@ -599,7 +685,7 @@ cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
     }
     if (MODE == kLinear) {
       for (int i = 0; i < p.phases; ++i)
-        ok = ok && (B_MN ? map_of(&p.b[i], g.bf16, g.b[i], 64, kBK) : map_of(&p.b[i], g.bf16, g.b[i], kBK, NT));
+        ok = ok && (B_MN ? map_of(&p.b[i], g.bf16, g.b[i], 64, kBK) : map_of(&p.b[i], g.bf16, g.b[i], kBK, NT / CG));
       if (g.y_tma) ok = ok && map_of(&p.out[0], g.bf16, g.out[0], 64, 128);
     } else {
       for (int i = 0; i < 2; ++i) ok = ok && map_of(&p.b[i], g.bf16, g.b[i], kBK, NT);
@@ -618,11 +704,22 @@ cudaError_t launch(const GemmArgs& g, cudaStream_t stream) {
   p.splits = g.splits;
   p.add = g.add;
   p.status = g.status;
-  constexpr auto kern = ff_gemm_kernel<T, PARTS, OUT, MODE, NT, B_MN>;
+  constexpr auto kern = ff_gemm_kernel<T, PARTS, OUT, MODE, NT, B_MN, CG>;
   cudaError_t e = opt_in_smem<kern>(C::smem_bytes());
   if (e != cudaSuccess) return e;
-  const int sms = sm_count();
-  return launch_early(kern, dim3(p.tiles < sms ? p.tiles : sms), kThreads, C::smem_bytes(), stream, p);
+  const int groups = sm_count() / CG, ctas = (p.tiles < groups ? p.tiles : groups) * CG;
+  return launch_clusters(kern, dim3(ctas), kThreads, C::smem_bytes(), stream, CG, p);
+}
+
+template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN>
+cudaError_t launch(const GemmArgs& g, cudaStream_t s) {
+  // pairs where every result has more than one row tile (fp32, whose epilogues add up sums, gains nothing from them)
+  if constexpr (PARTS == 1) {
+    bool pairs = MODE != kWeight && g.a[0].rows > 128;
+    if (MODE == kWeight) pairs = weight_pairs(false, {g.a[0].cols, g.a[1].cols, g.a[2].cols});
+    if (pairs) return launch_group<T, PARTS, OUT, MODE, NT, B_MN, 2>(g, s);
+  }
+  return launch_group<T, PARTS, OUT, MODE, NT, B_MN, 1>(g, s);
 }
 
 // 256 columns a tile where every result has more than 128 (fp32: 128, for the sums in registers).
@@ -637,7 +734,7 @@ cudaError_t dispatch(const GemmArgs& g, cudaStream_t s) {
   constexpr int kWide = PARTS == 3 ? 128 : 256;
   switch (g.mode) {
     case kGate: return launch<T, PARTS, OUT, kGate, kWide / 2, false>(g, s);
-    case kHidden: return launch<T, PARTS, OUT, kHidden, 64, false>(g, s);
+    case kHidden: return launch<T, PARTS, OUT, kHidden, PARTS == 3 ? 64 : 128, false>(g, s);
     case kLinear: {
       const bool wide = wide_tiles(PARTS == 3, {g.b_mn ? g.b[0].cols : g.b[0].rows});
       if (g.b_mn) return wide ? launch<T, PARTS, OUT, kLinear, kWide, true>(g, s) : launch<T, PARTS, OUT, kLinear, 128, true>(g, s);
@@ -660,8 +757,10 @@ cudaError_t gemm(const GemmArgs& g, cudaStream_t s) {
 // are counted as 1/32 of a round); at least 256 rows a split.
 int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms) {
   const bool wide = wide_tiles(f32, {n[0], n[1], n[2]});
+  const int cg = weight_pairs(f32, {m[0], m[1], m[2]}) ? 2 : 1;
   int64_t tiles = 0;
-  for (int j = 0; j < 3; ++j) tiles += tiles_of(m[j], 128) * tiles_of(n[j], wide ? 256 : 128);
+  for (int j = 0; j < 3; ++j) tiles += tiles_of(m[j], 128 * cg) * tiles_of(n[j], wide ? 256 : 128);
+  sms /= cg;
   int best = 1;
   float cost = 1e30f;
   for (int s = 1; s <= 32 && (s == 1 || rows / s >= 256); ++s) {

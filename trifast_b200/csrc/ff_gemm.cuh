@@ -30,7 +30,7 @@ struct GemmArgs {
   bool bf16;         // type of the 16-bit elements
   bool b_mn;         // kLinear: B is (K, N), N contiguous (else (N, K), K contiguous)
   int products;      // kLinear: 1 or 2 (their sum)
-  Matrix a[3], b[3]; // kGate: a0 = X, b = Wg, Wu.  kHidden: a0 = X, a1 = dY, b = Wg, Wu, Wd
+  Matrix a[3], b[3]; // kGate: a0 = X, b = Wg, Wu.  kHidden: a0 = dY, a1 = X, b = Wg, Wu, Wd
   Matrix out[3];     // kGate: h.  kHidden: da, db, h.  kLinear: y, in the call's own type
   bool y_tma;        // TMA can write y
   // kWeight: partial sums (splits, m0 * n0 + m1 * n1 + m2 * n2) fp32; added to what is there if `add`
@@ -46,8 +46,9 @@ int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, in
 
 // dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of `dtype`)
 cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Matrix& dst, cudaStream_t s);
-// dst[i] = sum over `splits` of partials[split * stride + i], in `dtype`
-cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* dst, int64_t count, int dtype, cudaStream_t s);
+// The sums over `splits` of partials[split * stride + i], in `dtype`: count[0] of them to dst[0], the next to dst[1], ...
+cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* const (&dst)[3], const int64_t (&count)[3], int dtype,
+                         cudaStream_t s);
 
 }  // namespace ff
 }  // namespace trifast

@@ -50,15 +50,39 @@ __global__ void stage_kernel(const T* __restrict__ src, int64_t ld, int64_t rows
   }
 }
 
-// The splits are added in order, in fp32.
-template <typename T>
-__global__ void sum_partials_kernel(const float* __restrict__ partials, int splits, int64_t stride, T* __restrict__ dst, int64_t count) {
+// The splits are added in order, in fp32; a thread makes four neighbours where all counts are multiples of four.
+struct Results {
+  void* dst[3];
+  int64_t end[3];
+};
+template <typename T, int N>
+__global__ void __launch_bounds__(256) sum_partials_kernel(const float* __restrict__ partials, int splits, int64_t stride, Results r) {
   after_previous();
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x) {
-    float s = 0.f;
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * N; i < r.end[2]; i += (int64_t)gridDim.x * blockDim.x * N) {
+    float s[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = 0.f;
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) s += partials[k * stride + i];
-    dst[i] = from_f32<T>(s);
+    for (int k = 0; k < splits; ++k) {
+      if constexpr (N == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(partials + k * stride + i);
+        s[0] += v.x;
+        s[1] += v.y;
+        s[2] += v.z;
+        s[3] += v.w;
+      } else {
+        s[0] += partials[k * stride + i];
+      }
+    }
+    const int at = i < r.end[0] ? 0 : i < r.end[1] ? 1 : 2;
+    T* dst = reinterpret_cast<T*>(at == 0 ? r.dst[0] : at == 1 ? r.dst[1] : r.dst[2]) + (i - (at == 0 ? 0 : at == 1 ? r.end[0] : r.end[1]));
+    if constexpr (N == 4 && std::is_same<T, float>::value) {
+      *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[1], s[2], s[3]);
+    } else if constexpr (N == 4) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack2<T>(s[0], s[1]), tc::pack2<T>(s[2], s[3]));
+    } else {
+      *dst = from_f32<T>(s[0]);
+    }
   }
 }
 
@@ -76,12 +100,25 @@ cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Ma
   return launch_early(stage_kernel<__half>, grid_for(threads), 256, 0, s, (const __half*)src, ld, rows, dst);
 }
 
-cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* dst, int64_t count, int dtype, cudaStream_t s) {
-  const dim3 g = grid_for(count);
+template <typename T>
+cudaError_t sum_type(const float* partials, int splits, int64_t stride, const Results& r, bool four, cudaStream_t s) {
+  return four ? launch_early(sum_partials_kernel<T, 4>, grid_for(r.end[2] / 4), 256, 0, s, partials, splits, stride, r)
+              : launch_early(sum_partials_kernel<T, 1>, grid_for(r.end[2]), 256, 0, s, partials, splits, stride, r);
+}
+
+cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* const (&dst)[3], const int64_t (&count)[3], int dtype,
+                         cudaStream_t s) {
+  Results r = {};
+  bool four = true;
+  for (int j = 0; j < 3; ++j) {
+    r.dst[j] = dst[j];
+    r.end[j] = (j ? r.end[j - 1] : 0) + count[j];
+    four = four && count[j] % 4 == 0;
+  }
   switch (dtype) {
-    case TRIFAST_F32: return launch_early(sum_partials_kernel<float>, g, 256, 0, s, partials, splits, stride, (float*)dst, count);
-    case TRIFAST_BF16: return launch_early(sum_partials_kernel<__nv_bfloat16>, g, 256, 0, s, partials, splits, stride, (__nv_bfloat16*)dst, count);
-    default: return launch_early(sum_partials_kernel<__half>, g, 256, 0, s, partials, splits, stride, (__half*)dst, count);
+    case TRIFAST_F32: return sum_type<float>(partials, splits, stride, r, four, s);
+    case TRIFAST_BF16: return sum_type<__nv_bfloat16>(partials, splits, stride, r, four, s);
+    default: return sum_type<__half>(partials, splits, stride, r, four, s);
   }
 }
 
