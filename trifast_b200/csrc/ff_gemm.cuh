@@ -44,6 +44,17 @@ cudaError_t gemm(const GemmArgs& g, cudaStream_t s);
 // Row splits of a kWeight launch over `rows` rows whose products have m[i] x n[i] results.
 int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms);
 
+// The forward pass of at most kFewRows rows (ff_few.cu).  h: rows x pitch fp32, pitch a multiple of 8 that holds `hidden`.
+constexpr int kFewRows = 8;
+struct FewArgs {
+  const void *x, *wg, *wu, *wd;
+  void* y;
+  float* h;
+  int64_t ld;
+  int rows, width, hidden, width_out, pitch, dtype;
+};
+cudaError_t few_rows(const FewArgs& a, cudaStream_t s);
+
 // dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of `dtype`)
 cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Matrix& dst, cudaStream_t s);
 // The sums over `splits` of partials[split * stride + i], in `dtype`: count[0] of them to dst[0], the next to dst[1], ...
