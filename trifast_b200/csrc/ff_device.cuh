@@ -41,29 +41,10 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
+// An arrival at a barrier of either CTA.  (What it tells of is TMEM, read or written, which the tcgen05 fences order; the
+// arrival and the wait need no more than the scope of a CTA.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-// mbar_wait for arrivals from the other CTA of the pair.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  const long long t0 = clock64();
-#pragma unroll 1
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitCycles) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // Into this CTA's memory, counted by a barrier of either CTA of the pair (plain per-CTA loads).
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
@@ -78,6 +59,14 @@ __device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint64_t a_desc, u
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // One arrival at this barrier of both CTAs when every MMA issued so far by this thread is done.
@@ -172,11 +161,11 @@ __device__ __forceinline__ void grad_units(const float* a, const float* b, const
 }
 
 // `box_cols` x `box_rows` tiles of a matrix
-inline bool map_of(CUtensorMap* map, bool bf16, const Matrix& m, int box_cols, int box_rows) {
+inline bool map_of(CUtensorMap* map, bool bf16, const Matrix& m, int box_cols, int box_rows) {   // (128-byte swizzle; 64 for 32 columns)
   const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, (uint64_t)m.planes};
   const uint64_t st[2] = {(uint64_t)m.pitch * 2, (uint64_t)m.plane * 2};
   const uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
-  return make_tensor_map(map, bf16, 3, m.p, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  return make_tensor_map(map, bf16, 3, m.p, dims, st, box, box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace ff

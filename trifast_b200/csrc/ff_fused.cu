@@ -33,6 +33,7 @@ constexpr int kTile = 128 * 64 * 2;      // 128 rows x 64 columns
 
 struct Params {
   CUtensorMap x, dy, wg, wu, wd, out;
+  CUtensorMap wg_across, wu_across;   // dX: half the width of 64 units
   int64_t rows;
   int tiles, chunks;   // row tiles; chunks of hidden units
   void* y;                  // result rows for stores that TMA cannot make
@@ -58,17 +59,27 @@ __device__ __forceinline__ Smem smem_of(uint8_t* raw) {
   return {raw + (b - r), b};
 }
 
-__device__ __forceinline__ uint32_t start(const Smem& sm, bool owner) {
+// After the barriers have been set up: TMEM, and with pairs of CTAs (CG = 2) whether both go on (`go`).
+template <int CG>
+__device__ __forceinline__ uint32_t start(const Smem& sm, bool owner, bool given_up, bool* go) {
+  if (threadIdx.x == 0) *reinterpret_cast<volatile uint32_t*>(sm.g + 264) = given_up;
   if (owner) {
-    tmem_alloc(smem_u32(sm.tmem_slot()), 512);
-    tmem_relinquish();
+    if (CG == 2) {
+      tmem_alloc_pair(smem_u32(sm.tmem_slot()), 512);
+    } else {
+      tmem_alloc(smem_u32(sm.tmem_slot()), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();
   tc_fence_after();
+  *go = CG == 2 ? (load_cluster(in_cta(sm.base + 264, 0)) | load_cluster(in_cta(sm.base + 264, 1))) == 0 : !given_up;
   return *sm.tmem_slot();
 }
 
+template <int CG>
 __device__ __forceinline__ void finish(const Smem& sm, bool owner, uint32_t tmem, unsigned int* status) {
   tc_fence_before();
   __syncthreads();
@@ -79,9 +90,14 @@ __device__ __forceinline__ void finish(const Smem& sm, bool owner, uint32_t tmem
     if (threadIdx.x == 0) set_status(status, kStatusTimeoutFeedForward);
     __syncthreads();
   }
+  // (neither CTA of a pair goes before the other's last access to it)
+  if (CG == 2) cluster_sync();
   if (owner) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if (CG == 2)
+      tmem_dealloc_pair(tmem, 512);
+    else
+      tmem_dealloc(tmem, 512);
   }
 }
 
@@ -97,7 +113,7 @@ __device__ __forceinline__ void store_tile(const Params& p, const Smem& sm, uint
   if (p.y_tma) fence_async_smem();
   group_sync(id, 128);
   if (p.y_tma) {
-    if (row == 0 && col < p.cols) {
+    if (row == 0 && col < p.cols && m0 < p.rows) {
       tma_store_3d(&p.out, sm.base + off, col, m0, 0);
       bulk_commit();
     }
@@ -112,63 +128,79 @@ __device__ __forceinline__ void store_tile(const Params& p, const Smem& sm, uint
   }
 }
 
-// Rings of the kernels that stream the weights: three chunks of Wg and Wu, two of Wd.
-constexpr int kGU = 3, kD = 2;
-template <int CP>
-struct Rows {
-  static constexpr int kBlocks = CP / 64;
-  static constexpr int kX = kBlocks * kTile;          // X or dY tile
-  static constexpr int kGuBytes = kBlocks * kTile;    // 64 rows of Wg and 64 of Wu
-  static constexpr int kDBytes = CP * 128;
-  static constexpr int kXOff = 1024, kGuOff = kXOff + 2 * kX, kDOff = kGuOff + kGU * kGuBytes, kOutOff = kDOff + kD * kDBytes;
-  static constexpr int smem_bytes() { return 1024 + kOutOff + 2 * kTile; }
-  static_assert(smem_bytes() <= kSmemLimit, "shared memory");
-};
-
-template <int CP>
-__device__ __forceinline__ void load_gu(const Params& p, uint32_t dst, uint32_t bar, int chunk) {
-#pragma unroll
-  for (int kb = 0; kb < CP / 64; ++kb) {
-    tma_load_3d(dst + kb * kTile, &p.wg, bar, kb * 64, chunk * kChunk, 0);
-    tma_load_3d(dst + kb * kTile + kTile / 2, &p.wu, bar, kb * 64, chunk * kChunk, 0);
-  }
-}
 template <int CP>
 __device__ __forceinline__ void load_rows(const CUtensorMap* map, uint32_t dst, uint32_t bar, int m0) {
 #pragma unroll
   for (int kb = 0; kb < CP / 64; ++kb) tma_load_3d(dst + kb * kTile, map, bar, kb * 64, m0, 0);
 }
-// S = X [Wg; Wu]^T, 128 x 128
+
+// ------------------------------------------------------------------ the kernels that keep rows
+// Two CTAs share every MMA, M = 256: each has a row tile of its own, its half of the weights' tiles (Wg's rows in the
+// first, Wu's in the second; half of what the other products have for columns) and its part of the results.  With one
+// CTA an MMA, each fetched all weights, 3.2 GB from L2 in 345 us for 1,048,576 rows forward, and read them from its
+// shared memory, which set the pace of dX (566 us).
+//
+// Warps: 0-7 elementwise, 8-11 results, 12 and 13 TMA (rows, Wg and Wu; Wd), 14 and 15, of the pair's first CTA, MMA
+// issuers (S and dH; the products of h, da and db).  A wait costs an issuer or producer about 100 cycles even for what is
+// there, so the two kinds of each do not share a warp.
+constexpr int kRowThreads = 512, kOutWarp = 8, kTmaWarp = 12, kTmaDWarp = 13, kSWarp = 14, kMmaWarp = 15;
+
+// Shared memory by kernel: rows (two X tiles, or X and dY), rings of chunks, result tiles.
+template <int CP, bool DX>
+struct Rows {
+  static constexpr int kBlocks = CP / 64, kHalf = CP / 2;
+  static constexpr int kX = kBlocks * kTile;
+  static constexpr int kSBytes = kBlocks * (kTile / 2);            // 64 rows of Wg or Wu, along their width
+  static constexpr int kAcross = kChunk * kHalf * 2;               // half the width of 64 rows of Wg (then of Wu), for dX
+  static constexpr int kGuBytes = kSBytes + (DX ? 2 * kAcross : 0);
+  static constexpr int kDBytes = DX ? CP * 64 : kHalf * 128;       // Wd: 32 units of all rows; 64 units of half the rows
+  static constexpr int kGU = DX ? 3 : 4, kD = DX ? 3 : 4;
+  static constexpr int kXOff = 1024, kGuOff = kXOff + 2 * kX, kDOff = kGuOff + kGU * kGuBytes, kOutOff = kDOff + kD * kDBytes;
+  static constexpr int smem_bytes() { return 1024 + kOutOff + 2 * kTile; }
+  static_assert(smem_bytes() <= kSmemLimit && kGuBytes % 1024 == 0 && kDBytes % 1024 == 0, "shared memory");
+};
+
+// The row tiles of a CTA, and the chunks of hidden units that it walks over all of them.
+struct Walk {
+  int rank, first, stride, items, total;
+  __device__ __forceinline__ Walk(const Params& p) {
+    rank = (int)cluster_rank();
+    first = blockIdx.x / 2;
+    stride = gridDim.x / 2;
+    const int pairs = (p.tiles + 1) / 2;
+    items = first < pairs ? (pairs - 1 - first) / stride + 1 : 0;
+    total = items * p.chunks;
+  }
+  __device__ __forceinline__ int row(int it) const { return ((first + it * stride) * 2 + rank) * 128; }
+};
+
+// Producers: this CTA's part, counted by the first CTA's barrier, which expects both parts.
+struct Filler {
+  uint32_t base, counted;   // this CTA's barriers, the first CTA's
+  int rank;
+  __device__ __forceinline__ uint32_t expect(int bar, int bytes) const {
+    if (rank == 0) mbar_arrive_expect_tx(base + 8u * bar, 2 * bytes);
+    return counted + 8u * bar;
+  }
+};
+
+// S = X [Wg; Wu]^T, 256 x 128
 template <bool BF16, int CP>
-__device__ __forceinline__ void mma_s(uint32_t d, uint32_t x, uint32_t gu) {
+__device__ __forceinline__ void pair_s(uint32_t d, uint32_t x, uint32_t gu) {
   const uint64_t ad = make_smem_desc(x, 16, 1024, kSwizzle128), bd = make_smem_desc(gu, 16, 1024, kSwizzle128);
 #pragma unroll
-  for (int k = 0; k < CP / 16; ++k) {
-    const uint32_t off = (k >> 2) * (kTile >> 4) + (k & 3) * 2;
-    umma_ss(d, ad + off, bd + off, make_idesc(128, 128, BF16, false, false), k > 0);
-  }
-}
-// dH = dY Wd, 128 x 64
-template <bool BF16, int CP>
-__device__ __forceinline__ void mma_dh(uint32_t d, uint32_t dy, uint32_t wd) {
-  const uint64_t ad = make_smem_desc(dy, 16, 1024, kSwizzle128), bd = make_smem_desc(wd, 16, 1024, kSwizzle128);
-#pragma unroll
   for (int k = 0; k < CP / 16; ++k)
-    umma_ss(d, ad + (k >> 2) * (kTile >> 4) + (k & 3) * 2, bd + k * (2048 >> 4), make_idesc(128, 64, BF16, false, true), k > 0);
+    umma_ss_pair(d, ad + (k >> 2) * (kTile >> 4) + (k & 3) * 2, bd + (k >> 2) * (kTile >> 5) + (k & 3) * 2,
+                 make_idesc(256, 128, BF16, false, false), k > 0);
 }
-
-// Warps of the kernels that keep rows: 0-7 elementwise (two warpgroups, which take the chunks in turn), 8-11 results,
-// 12 and 13 TMA (rows, Wg and Wu; Wd), 14 and 15 MMA issuers (S and dH; the products of h, da and db).  A wait costs an
-// issuer or producer about 100 cycles even for what is there, so the two kinds of each do not share a warp.
-constexpr int kRowThreads = 512, kOutWarp = 8, kTmaWarp = 12, kTmaDWarp = 13, kSWarp = 14, kMmaWarp = 15;
 
 // The 128 x CP sums of an item at column `acc` of TMEM, as result rows: warps 8-11, once per item.
 template <typename T, int CP>
-__device__ __forceinline__ void write_results(const Params& p, const Smem& sm, uint32_t acc, int done, int free) {
+__device__ __forceinline__ void write_results(const Params& p, const Smem& sm, const Walk& walk, uint32_t acc, uint32_t out_off, int done,
+                                              uint32_t free) {
   const int lane = threadIdx.x & 31, wq = (threadIdx.x >> 5) & 3;
   const uint32_t at = acc + ((uint32_t)(wq * 32) << 16);
-  int it = 0;
-  for (int w = blockIdx.x; w < p.tiles; w += gridDim.x, ++it) {
+  for (int it = 0; it < walk.items; ++it) {
     // all go on or none: store_tile has barriers
     if (!group_all(1, 128, mbar_wait(sm.bar(done), it & 1, sm.abort_flag()))) break;
     tc_fence_after();
@@ -183,21 +215,20 @@ __device__ __forceinline__ void write_results(const Params& p, const Smem& sm, u
     }
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(sm.bar(free));
+    if (lane == 0) mbar_arrive_cluster(free);
 #pragma unroll
-    for (int c = 0; c < CP; c += 64) store_tile(p, sm, Rows<CP>::kOutOff + (c >> 6) * kTile, 1, u + (c >> 1), w * 128, c);
+    for (int c = 0; c < CP; c += 64) store_tile(p, sm, out_off + (c >> 6) * kTile, 1, u + (c >> 1), walk.row(it), c);
   }
   bulk_wait();
 }
 
 // ------------------------------------------------------------------ forward
-// An item is one row tile.  TMEM: three S of 128 columns, which the chunks take in turn (h over a's first columns), so
-// that the tensor pipe is two chunks ahead of the gates; Y [384, 384 + CP).
-// With S of two row tiles in two buffers (half the weight traffic) a chunk waited for its own gate, 132 us for
-// 303,104 rows at width 128, hidden 512.
+// TMEM: three S of 128 columns, which the chunks take in turn (h over a's first columns), so that the tensor pipe is two
+// chunks ahead of the gates; Y [384, 384 + CP).
 template <typename T, int CP>
 __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid_constant__ Params p) {
-  using L = Rows<CP>;
+  using L = Rows<CP, false>;
+  constexpr int kGU = L::kGU, kD = L::kD;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int X_FULL = 0, X_EMPTY = 2, GU_FULL = 4, GU_EMPTY = GU_FULL + kGU, D_FULL = GU_EMPTY + kGU, D_EMPTY = D_FULL + kD,
                 S_FULL = D_EMPTY + kD, H_READY = S_FULL + 3, H_FREE = H_READY + 3, Y_DONE = H_FREE + 3, Y_FREE = Y_DONE + 1, NBARS = Y_FREE + 1;
@@ -206,30 +237,36 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
   const Smem sm = smem_of(smem_raw);
   volatile int* abort_flag = sm.abort_flag();
   after_previous();
-  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+  const bool given_up = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), (i >= H_READY && i < H_READY + 3) || i == Y_FREE ? 4 : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), (i >= H_READY && i < H_READY + 3) || i == Y_FREE ? 8 : 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
-  const uint32_t tmem = start(sm, warp == kMmaWarp);
-  const int n = p.chunks;
-  const int total = (int)blockIdx.x < p.tiles ? ((p.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * n : 0;   // chunks of this CTA
+  bool go;
+  const uint32_t tmem = start<2>(sm, warp == kMmaWarp, given_up, &go);
+  const Walk walk(p);
+  const int n = p.chunks, total = go ? walk.total : 0;
+  const uint32_t first = in_cta(sm.base, 0);   // the first CTA's barriers
+  const Filler fill{sm.base, first, walk.rank};
   auto wait = [&](int b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(sm.bar(b), parity, abort_flag)); };
   auto x_tile = [&](int it) { return sm.base + L::kXOff + (it & 1) * L::kX; };
   auto gu_tile = [&](int g) { return sm.base + L::kGuOff + (g % kGU) * L::kGuBytes; };
   auto d_tile = [&](int g) { return sm.base + L::kDOff + (g % kD) * L::kDBytes; };
 
-  if (warp == kTmaWarp) {
+  if (!go) {
+  } else if (warp == kTmaWarp) {
     bool ok = true;
+    const CUtensorMap* own = walk.rank == 0 ? &p.wg : &p.wu;
     for (int g = 0, c = 0, it = 0; g < total && ok; ++g, c = c + 1 == n ? 0 : c + 1) {
       if (c == 0) {
         if (it >= 2) ok = wait(X_EMPTY + (it & 1), (it / 2 - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
-          mbar_arrive_expect_tx(sm.bar(X_FULL + (it & 1)), L::kX);
-          load_rows<CP>(&p.x, x_tile(it), sm.bar(X_FULL + (it & 1)), (blockIdx.x + it * gridDim.x) * 128);
+          const uint32_t f = fill.expect(X_FULL + (it & 1), L::kX);
+#pragma unroll
+          for (int kb = 0; kb < L::kBlocks; ++kb) tma_load_3d_pair(x_tile(it) + kb * kTile, &p.x, f, kb * 64, walk.row(it), 0);
         }
         __syncwarp();
         ++it;
@@ -237,8 +274,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
       if (g >= kGU) ok = wait(GU_EMPTY + g % kGU, (g / kGU - 1) & 1);
       if (!ok) break;
       if (elect_one()) {
-        mbar_arrive_expect_tx(sm.bar(GU_FULL + g % kGU), L::kGuBytes);
-        load_gu<CP>(p, gu_tile(g), sm.bar(GU_FULL + g % kGU), c);
+        const uint32_t f = fill.expect(GU_FULL + g % kGU, L::kGuBytes);
+#pragma unroll
+        for (int kb = 0; kb < L::kBlocks; ++kb) tma_load_3d_pair(gu_tile(g) + kb * (kTile / 2), own, f, kb * 64, c * kChunk, 0);
       }
       __syncwarp();
     }
@@ -247,25 +285,22 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
     for (int g = 0, c = 0; g < total && ok; ++g, c = c + 1 == n ? 0 : c + 1) {
       if (g >= kD) ok = wait(D_EMPTY + g % kD, (g / kD - 1) & 1);
       if (!ok) break;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(sm.bar(D_FULL + g % kD), L::kDBytes);
-        tma_load_3d(d_tile(g), &p.wd, sm.bar(D_FULL + g % kD), c * kChunk, 0, 0);
-      }
+      if (elect_one()) tma_load_3d_pair(d_tile(g), &p.wd, fill.expect(D_FULL + g % kD, L::kDBytes), c * kChunk, walk.rank * L::kHalf, 0);
       __syncwarp();
     }
   } else if (warp == kSWarp) {
     bool ok = true;
-    for (int g = 0, c = 0, it = 0; g < total && ok; ++g) {
+    for (int g = 0, c = 0, it = 0; g < total && ok && walk.rank == 0; ++g) {
       if (c == 0) ok = wait(X_FULL + (it & 1), (it >> 1) & 1);
       ok = ok && wait(GU_FULL + g % kGU, (g / kGU) & 1);
       if (ok && g >= 3) ok = wait(H_FREE + g % 3, (g / 3 - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        mma_s<kBf16, CP>(tmem + (g % 3) * 128, x_tile(it), gu_tile(g));
-        umma_commit(sm.bar(S_FULL + g % 3));
-        umma_commit(sm.bar(GU_EMPTY + g % kGU));
-        if (c == n - 1) umma_commit(sm.bar(X_EMPTY + (it & 1)));
+        pair_s<kBf16, CP>(tmem + (g % 3) * 128, x_tile(it), gu_tile(g));
+        umma_commit_pair(sm.bar(S_FULL + g % 3));
+        umma_commit_pair(sm.bar(GU_EMPTY + g % kGU));
+        if (c == n - 1) umma_commit_pair(sm.bar(X_EMPTY + (it & 1)));
       }
       __syncwarp();
       if (++c == n) {
@@ -275,7 +310,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
     }
   } else if (warp == kMmaWarp) {
     bool ok = true;
-    for (int g = 0, c = 0, it = 0; g < total && ok; ++g) {
+    for (int g = 0, c = 0, it = 0; g < total && ok && walk.rank == 0; ++g) {
       ok = wait(D_FULL + g % kD, (g / kD) & 1) && wait(H_READY + g % 3, (g / 3) & 1);
       if (ok && c == 0 && it > 0) ok = wait(Y_FREE, (it - 1) & 1);
       if (!ok) break;
@@ -284,10 +319,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
         const uint64_t bd = make_smem_desc(d_tile(g), 16, 1024, kSwizzle128);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_ts(tmem + 384, tmem + (g % 3) * 128 + k * 8, bd + k * 2, make_idesc(128, CP, kBf16, false, false), (c > 0 || k > 0) ? 1u : 0u);
-        umma_commit(sm.bar(H_FREE + g % 3));
-        umma_commit(sm.bar(D_EMPTY + g % kD));
-        if (c == n - 1) umma_commit(sm.bar(Y_DONE));
+          umma_ts_pair(tmem + 384, tmem + (g % 3) * 128 + k * 8, bd + k * 2, make_idesc(256, CP, kBf16, false, false), (c > 0 || k > 0) ? 1u : 0u);
+        umma_commit_pair(sm.bar(H_FREE + g % 3));
+        umma_commit_pair(sm.bar(D_EMPTY + g % kD));
+        if (c == n - 1) umma_commit_pair(sm.bar(Y_DONE));
       }
       __syncwarp();
       if (++c == n) {
@@ -296,23 +331,25 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
       }
     }
   } else if (warp >= kOutWarp) {
-    write_results<T, CP>(p, sm, tmem + 384, Y_DONE, Y_FREE);
+    write_results<T, CP>(p, sm, walk, tmem + 384, L::kOutOff, Y_DONE, first + 8u * Y_FREE);
   } else {
+    // (the warpgroups take the chunks in turn; half of every chunk each made a shorter chain from one use of a buffer to
+    // the next and 361 us of 336)
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     for (int g = warp >> 2; g < total; g += 2) {
       if (!wait(S_FULL + g % 3, (g / 3) & 1)) break;
       tc_fence_after();
       const uint32_t ts = lanes + (g % 3) * 128;
       float a[2][16], b[2][16];
-      tmem_ld16(ts, reinterpret_cast<uint32_t*>(a[0]));
-      tmem_ld16(ts + 64, reinterpret_cast<uint32_t*>(b[0]));
+      auto load = [&](int i) {
+        tmem_ld16(ts + 16 * i, reinterpret_cast<uint32_t*>(a[i & 1]));
+        tmem_ld16(ts + 64 + 16 * i, reinterpret_cast<uint32_t*>(b[i & 1]));
+      };
+      load(0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // 16 units at a time, the next ones on their way
         tmem_wait_ld();
-        if (i < 3) {
-          tmem_ld16(ts + 16 * (i + 1), reinterpret_cast<uint32_t*>(a[(i + 1) & 1]));
-          tmem_ld16(ts + 64 + 16 * (i + 1), reinterpret_cast<uint32_t*>(b[(i + 1) & 1]));
-        }
+        if (i < 3) load(i + 1);
         uint32_t h[8];
         gate_units<T, 16>(a[i & 1], b[i & 1], h);
         tmem_st8(ts + 8 * i, h);
@@ -320,18 +357,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(H_READY + g % 3));
+      if (lane == 0) mbar_arrive_cluster(first + 8u * (H_READY + g % 3));
     }
   }
-  finish(sm, warp == kMmaWarp, tmem, p.status);
+  finish<2>(sm, warp == kMmaWarp, tmem, p.status);
 }
 
 // ------------------------------------------------------------------ dX
-// An item is one row tile; the chunks alternate between two buffers of TMEM, [0, 192) and [192, 384): S and dH, with da
-// over a's columns and db over b's (16 columns of each 32); dX [384, 384 + CP).
+// The chunks alternate between two buffers of TMEM, [0, 192) and [192, 384): S and dH, with da and db over dH's columns (16
+// and 16 of each 32), so that the next S only waits for a and b to be read; dX [384, 384 + CP).
 template <typename T, int CP>
 __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_constant__ Params p) {
-  using L = Rows<CP>;
+  using L = Rows<CP, true>;
+  constexpr int kGU = L::kGU, kD = L::kD;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int XY_FULL = 0, XY_EMPTY = 1, GU_FULL = 2, GU_EMPTY = GU_FULL + kGU, D_FULL = GU_EMPTY + kGU, D_EMPTY = D_FULL + kD,
                 S_FULL = D_EMPTY + kD, P_READY = S_FULL + 2, P_FREE = P_READY + 2, DX_DONE = P_FREE + 2, DX_FREE = DX_DONE + 1, NBARS = DX_FREE + 1;
@@ -340,39 +378,44 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
   const Smem sm = smem_of(smem_raw);
   volatile int* abort_flag = sm.abort_flag();
   after_previous();
-  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+  const bool given_up = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), i == DX_FREE ? 4 : (i >= P_READY && i < P_READY + 2) ? 8 : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), i == DX_FREE ? 8 : (i >= P_READY && i < P_READY + 2) ? 16 : 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
-  const uint32_t tmem = start(sm, warp == kMmaWarp);
-  const int n = p.chunks;
-  const int total = (int)blockIdx.x < p.tiles ? ((p.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * n : 0;   // chunks of this CTA
+  bool go;
+  const uint32_t tmem = start<2>(sm, warp == kMmaWarp, given_up, &go);
+  const Walk walk(p);
+  const int n = p.chunks, total = go ? walk.total : 0;
+  const uint32_t first = in_cta(sm.base, 0);   // the first CTA's barriers
+  const Filler fill{sm.base, first, walk.rank};
   const uint32_t x_tile = sm.base + L::kXOff, dy_tile = x_tile + L::kX;
   auto wait = [&](int b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(sm.bar(b), parity, abort_flag)); };
   auto gu_tile = [&](int g) { return sm.base + L::kGuOff + (g % kGU) * L::kGuBytes; };
   auto d_tile = [&](int g) { return sm.base + L::kDOff + (g % kD) * L::kDBytes; };
 
-  if (warp == kTmaWarp) {
+  if (!go) {
+  } else if (warp == kTmaWarp) {
     bool ok = true;
+    const CUtensorMap* own = walk.rank == 0 ? &p.wg : &p.wu;
     for (int g = 0, c = 0, it = 0; g < total && ok; ++g, c = c + 1 == n ? 0 : c + 1) {
       if (c == 0) {
         if (it > 0) ok = wait(XY_EMPTY, (it - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
-          const int row = (blockIdx.x + it * gridDim.x) * 128, next = row + gridDim.x * 128;
-          mbar_arrive_expect_tx(sm.bar(XY_FULL), 2 * L::kX);
-          load_rows<CP>(&p.x, x_tile, sm.bar(XY_FULL), row);
-          load_rows<CP>(&p.dy, dy_tile, sm.bar(XY_FULL), row);
-          // (one buffer of rows: the next ones are fetched from L2)
-          if (g + n < total)
+          const uint32_t f = fill.expect(XY_FULL, 2 * L::kX);
 #pragma unroll
-            for (int kb = 0; kb < CP / 64; ++kb) {
-              tma_prefetch_3d(&p.x, kb * 64, next, 0);
-              tma_prefetch_3d(&p.dy, kb * 64, next, 0);
+          for (int kb = 0; kb < L::kBlocks; ++kb) {
+            tma_load_3d_pair(x_tile + kb * kTile, &p.x, f, kb * 64, walk.row(it), 0);
+            tma_load_3d_pair(dy_tile + kb * kTile, &p.dy, f, kb * 64, walk.row(it), 0);
+            // (one buffer of rows: the next ones are fetched from L2)
+            if (it + 1 < walk.items) {
+              tma_prefetch_3d(&p.x, kb * 64, walk.row(it + 1), 0);
+              tma_prefetch_3d(&p.dy, kb * 64, walk.row(it + 1), 0);
             }
+          }
         }
         __syncwarp();
         ++it;
@@ -380,8 +423,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
       if (g >= kGU) ok = wait(GU_EMPTY + g % kGU, (g / kGU - 1) & 1);
       if (!ok) break;
       if (elect_one()) {
-        mbar_arrive_expect_tx(sm.bar(GU_FULL + g % kGU), L::kGuBytes);
-        load_gu<CP>(p, gu_tile(g), sm.bar(GU_FULL + g % kGU), c);
+        const uint32_t f = fill.expect(GU_FULL + g % kGU, L::kGuBytes), across = gu_tile(g) + L::kSBytes;
+#pragma unroll
+        for (int kb = 0; kb < L::kBlocks; ++kb) tma_load_3d_pair(gu_tile(g) + kb * (kTile / 2), own, f, kb * 64, c * kChunk, 0);
+        tma_load_3d_pair(across, &p.wg_across, f, walk.rank * L::kHalf, c * kChunk, 0);
+        tma_load_3d_pair(across + L::kAcross, &p.wu_across, f, walk.rank * L::kHalf, c * kChunk, 0);
       }
       __syncwarp();
     }
@@ -390,31 +436,33 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
     for (int g = 0, c = 0; g < total && ok; ++g, c = c + 1 == n ? 0 : c + 1) {
       if (g >= kD) ok = wait(D_EMPTY + g % kD, (g / kD - 1) & 1);
       if (!ok) break;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(sm.bar(D_FULL + g % kD), L::kDBytes);
-        tma_load_3d(d_tile(g), &p.wd, sm.bar(D_FULL + g % kD), c * kChunk, 0, 0);
-      }
+      if (elect_one()) tma_load_3d_pair(d_tile(g), &p.wd, fill.expect(D_FULL + g % kD, L::kDBytes), c * kChunk + walk.rank * 32, 0, 0);
       __syncwarp();
     }
   } else if (warp == kSWarp) {
     bool ok = true;
-    for (int g = 0, c = 0, it = 0; g < total && ok; ++g) {
+    for (int g = 0, c = 0, it = 0; g < total && ok && walk.rank == 0; ++g) {
       if (c == 0) ok = wait(XY_FULL, it & 1);
       ok = ok && wait(GU_FULL + g % kGU, (g / kGU) & 1);
-      if (ok && g >= 2) ok = wait(P_FREE + (g & 1), ((g >> 1) - 1) & 1);
+      if (ok && g >= 2) ok = wait(P_READY + (g & 1), ((g >> 1) - 1) & 1);   // (a and b have been read)
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem + (g & 1) * 192;
-      if (elect_one()) mma_s<kBf16, CP>(d, x_tile, gu_tile(g));
+      if (elect_one()) pair_s<kBf16, CP>(d, x_tile, gu_tile(g));
       __syncwarp();
       ok = wait(D_FULL + g % kD, (g / kD) & 1);
+      if (ok && g >= 2) ok = wait(P_FREE + (g & 1), ((g >> 1) - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        mma_dh<kBf16, CP>(d + 128, dy_tile, d_tile(g));
-        umma_commit(sm.bar(S_FULL + (g & 1)));
-        umma_commit(sm.bar(D_EMPTY + g % kD));
-        if (c == n - 1) umma_commit(sm.bar(XY_EMPTY));
+        // dH = dY Wd, 256 x 64; Wd across, halves of 32 units (rows of 64 bytes)
+        const uint64_t ad = make_smem_desc(dy_tile, 16, 1024, kSwizzle128), bd = make_smem_desc(d_tile(g), 512, 512, kSwizzle64);
+#pragma unroll
+        for (int k = 0; k < CP / 16; ++k)
+          umma_ss_pair(d + 128, ad + (k >> 2) * (kTile >> 4) + (k & 3) * 2, bd + k * (1024 >> 4), make_idesc(256, 64, kBf16, false, true), k > 0);
+        umma_commit_pair(sm.bar(S_FULL + (g & 1)));
+        umma_commit_pair(sm.bar(D_EMPTY + g % kD));
+        if (c == n - 1) umma_commit_pair(sm.bar(XY_EMPTY));
       }
       __syncwarp();
       if (++c == n) {
@@ -424,24 +472,27 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
     }
   } else if (warp == kMmaWarp) {
     bool ok = true;
-    for (int g = 0, c = 0, it = 0; g < total && ok; ++g) {
-      // (its Wg and Wu are there: S has read them)
+    for (int g = 0, c = 0, it = 0; g < total && ok && walk.rank == 0; ++g) {
+      // (its Wg and Wu are there: they came with those that S was made of)
       ok = wait(P_READY + (g & 1), (g >> 1) & 1);
       if (ok && c == 0 && it > 0) ok = wait(DX_FREE, (it - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t a = tmem + (g & 1) * 192, gu = gu_tile(g);
-        // (units down, width across: 64-column blocks kTile apart)
-        const uint64_t bg = make_smem_desc(gu, kTile, 1024, kSwizzle128), bu = make_smem_desc(gu + kTile / 2, kTile, 1024, kSwizzle128);
-        constexpr uint32_t idesc = make_idesc(128, CP, kBf16, false, true);
+        // B: units down, half the width across
+        constexpr uint32_t kRow = L::kHalf * 2;
+        constexpr uint64_t kSwz = L::kHalf == 64 ? kSwizzle128 : kSwizzle64;
+        constexpr uint32_t idesc = make_idesc(256, CP, kBf16, false, true);
+        const uint32_t a = tmem + (g & 1) * 192 + 128, w = gu_tile(g) + L::kSBytes;
+        const uint64_t bg = make_smem_desc(w, 8 * kRow, 8 * kRow, kSwz), bu = make_smem_desc(w + L::kAcross, 8 * kRow, 8 * kRow, kSwz);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_ts(tmem + 384, a + (k >> 1) * 32 + (k & 1) * 8, bg + k * (2048 >> 4), idesc, (c > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k)
+          umma_ts_pair(tmem + 384, a + (k >> 1) * 32 + (k & 1) * 8, bg + k * (16 * kRow >> 4), idesc, (c > 0 || k > 0) ? 1u : 0u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_ts(tmem + 384, a + 64 + (k >> 1) * 32 + (k & 1) * 8, bu + k * (2048 >> 4), idesc, 1u);
-        umma_commit(sm.bar(P_FREE + (g & 1)));
-        umma_commit(sm.bar(GU_EMPTY + g % kGU));
-        if (c == n - 1) umma_commit(sm.bar(DX_DONE));
+        for (int k = 0; k < 4; ++k) umma_ts_pair(tmem + 384, a + 16 + (k >> 1) * 32 + (k & 1) * 8, bu + k * (16 * kRow >> 4), idesc, 1u);
+        umma_commit_pair(sm.bar(P_FREE + (g & 1)));
+        umma_commit_pair(sm.bar(GU_EMPTY + g % kGU));
+        if (c == n - 1) umma_commit_pair(sm.bar(DX_DONE));
       }
       __syncwarp();
       if (++c == n) {
@@ -450,7 +501,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
       }
     }
   } else if (warp >= kOutWarp) {
-    write_results<T, CP>(p, sm, tmem + 384, DX_DONE, DX_FREE);
+    write_results<T, CP>(p, sm, walk, tmem + 384, L::kOutOff, DX_DONE, first + 8u * DX_FREE);
   } else {
     // both warpgroups take half the units of every chunk: its gradients are the longest link of the chain from one
     // use of a buffer to the next
@@ -475,17 +526,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
         uint32_t da[8], db[8];
         grad_units<T, 16, false>(a[i], b[i], dh[i], da, db, nullptr);
         if (i == 0) tmem_wait_ld();
-        // (over columns of a and b that this warp has read)
-        tmem_st8(ts + grp * 32 + 8 * i, da);
-        tmem_st8(ts + 64 + grp * 32 + 8 * i, db);
+        // (over columns of dH that this warp has read)
+        tmem_st8(ts + 128 + grp * 32 + 8 * i, da);
+        tmem_st8(ts + 128 + grp * 32 + 16 + 8 * i, db);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(P_READY + (g & 1)));
+      if (lane == 0) mbar_arrive_cluster(first + 8u * (P_READY + (g & 1)));
     }
   }
-  finish(sm, warp == kMmaWarp, tmem, p.status);
+  finish<2>(sm, warp == kMmaWarp, tmem, p.status);
 }
 
 // ------------------------------------------------------------------ dWg, dWu, dWd
@@ -501,6 +552,24 @@ struct Weights {   // (warps of this kernel: 0-7 elementwise, 8 TMA, 9 and 10 MM
   static constexpr int smem_bytes() { return 1024 + kStgOff + 3 * kTile; }
   static_assert(smem_bytes() <= kSmemLimit, "shared memory");
 };
+
+// S = X [Wg; Wu]^T, 128 x 128, and dH = dY Wd, 128 x 64, of one CTA
+template <bool BF16, int CP>
+__device__ __forceinline__ void mma_s(uint32_t d, uint32_t x, uint32_t gu) {
+  const uint64_t ad = make_smem_desc(x, 16, 1024, kSwizzle128), bd = make_smem_desc(gu, 16, 1024, kSwizzle128);
+#pragma unroll
+  for (int k = 0; k < CP / 16; ++k) {
+    const uint32_t off = (k >> 2) * (kTile >> 4) + (k & 3) * 2;
+    umma_ss(d, ad + off, bd + off, make_idesc(128, 128, BF16, false, false), k > 0);
+  }
+}
+template <bool BF16, int CP>
+__device__ __forceinline__ void mma_dh(uint32_t d, uint32_t dy, uint32_t wd) {
+  const uint64_t ad = make_smem_desc(dy, 16, 1024, kSwizzle128), bd = make_smem_desc(wd, 16, 1024, kSwizzle128);
+#pragma unroll
+  for (int k = 0; k < CP / 16; ++k)
+    umma_ss(d, ad + (k >> 2) * (kTile >> 4) + (k & 3) * 2, bd + k * (2048 >> 4), make_idesc(128, 64, BF16, false, true), k > 0);
+}
 
 template <typename T, int CP>
 __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constant__ Params p) {
@@ -519,7 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
     *abort_flag = 0;
     mbar_fence_init();
   }
-  const uint32_t tmem = start(sm, warp == 9);
+  bool go;
+  const uint32_t tmem = start<1>(sm, warp == 9, false, &go);
   const int chunk = blockIdx.x % p.chunks, split = blockIdx.x / p.chunks;
   const int lo = (int)((int64_t)p.tiles * split / p.splits), hi = (int)((int64_t)p.tiles * (split + 1) / p.splits);
   const uint32_t gu = sm.base + L::kWOff, wd = gu + L::kGuBytes, stg = sm.base + L::kStgOff;
@@ -530,7 +600,11 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
   if (warp == 8) {
     if (elect_one()) {
       mbar_arrive_expect_tx(sm.bar(W_FULL), L::kGuBytes + L::kDBytes);
-      load_gu<CP>(p, gu, sm.bar(W_FULL), chunk);
+#pragma unroll
+      for (int kb = 0; kb < CP / 64; ++kb) {
+        tma_load_3d(gu + kb * kTile, &p.wg, sm.bar(W_FULL), kb * 64, chunk * kChunk, 0);
+        tma_load_3d(gu + kb * kTile + kTile / 2, &p.wu, sm.bar(W_FULL), kb * 64, chunk * kChunk, 0);
+      }
       tma_load_3d(wd, &p.wd, sm.bar(W_FULL), chunk * kChunk, 0, 0);
     }
     __syncwarp();
@@ -686,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
       }
     }
   }
-  finish(sm, warp == 9, tmem, p.status);
+  finish<1>(sm, warp == 9, tmem, p.status);
 }
 
 int64_t tiles_of(int64_t x, int tile) { return (x + tile - 1) / tile; }
@@ -710,7 +784,8 @@ cudaError_t launch(const FusedArgs& g, cudaStream_t stream) {
   p.width_out = (int)g.wd.rows;
   p.status = g.status;
   bool ok = map_of(&p.x, g.bf16, g.x, 64, 128) && map_of(&p.wg, g.bf16, g.wg, 64, 64) && map_of(&p.wu, g.bf16, g.wu, 64, 64) &&
-            map_of(&p.wd, g.bf16, g.wd, 64, CP);
+            map_of(&p.wd, g.bf16, g.wd, g.what == kDx ? 32 : 64, g.what == kForward ? CP / 2 : CP);
+  if (g.what == kDx) ok = ok && map_of(&p.wg_across, g.bf16, g.wg, CP / 2, 64) && map_of(&p.wu_across, g.bf16, g.wu, CP / 2, 64);
   if (g.what != kForward) ok = ok && map_of(&p.dy, g.bf16, g.dy, 64, 128);
   if (g.what != kDw && g.y_tma) ok = ok && map_of(&p.out, g.bf16, g.out, 64, 128);
   if (!ok) return cudaErrorInvalidValue;
@@ -720,12 +795,14 @@ cudaError_t launch(const FusedArgs& g, cudaStream_t stream) {
     if ((e = opt_in_smem<ff_dw_kernel<T, CP>>(Weights<CP>::smem_bytes())) != cudaSuccess) return e;
     return launch_early(ff_dw_kernel<T, CP>, dim3((unsigned)(p.chunks * p.splits)), kThreads, Weights<CP>::smem_bytes(), stream, p);
   }
+  const int pairs = (p.tiles + 1) / 2;
+  const dim3 grid(2 * (pairs < sms / 2 ? pairs : sms / 2));
   if (g.what == kDx) {
-    if ((e = opt_in_smem<ff_dx_kernel<T, CP>>(Rows<CP>::smem_bytes())) != cudaSuccess) return e;
-    return launch_early(ff_dx_kernel<T, CP>, dim3((unsigned)(p.tiles < sms ? p.tiles : sms)), kRowThreads, Rows<CP>::smem_bytes(), stream, p);
+    if ((e = opt_in_smem<ff_dx_kernel<T, CP>>(Rows<CP, true>::smem_bytes())) != cudaSuccess) return e;
+    return launch_clusters(ff_dx_kernel<T, CP>, grid, kRowThreads, Rows<CP, true>::smem_bytes(), stream, 2, p);
   }
-  if ((e = opt_in_smem<ff_forward_kernel<T, CP>>(Rows<CP>::smem_bytes())) != cudaSuccess) return e;
-  return launch_early(ff_forward_kernel<T, CP>, dim3((unsigned)(p.tiles < sms ? p.tiles : sms)), kRowThreads, Rows<CP>::smem_bytes(), stream, p);
+  if ((e = opt_in_smem<ff_forward_kernel<T, CP>>(Rows<CP, false>::smem_bytes())) != cudaSuccess) return e;
+  return launch_clusters(ff_forward_kernel<T, CP>, grid, kRowThreads, Rows<CP, false>::smem_bytes(), stream, 2, p);
 }
 
 template <typename T>

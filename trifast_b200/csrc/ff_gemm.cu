@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
     uint32_t acc = tmem_base;
     auto wait_read = [&](int sum) {   // until the epilogue has read this sum
       const int e = ACC_EMPTY + (sum & 1), parity = (sum >> 1) & 1;
-      if (sum >= 0) ok = CG == 2 ? mbar_wait_cluster(bar(e), parity, abort_flag) : mbar_wait(bar(e), parity, abort_flag);
+      if (sum >= 0) ok = mbar_wait(bar(e), parity, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     };
