@@ -151,35 +151,37 @@ struct FfWeights {
   Matrix gate, up, down;
 };
 
-// The weights as the products read them, laid out anew where they have to be.
-int ff_weights(const trifast_ff* f, const FfPlan& p, char* ws, const void* wg, const void* wu, const void* wd,
-               FfWeights* out, cudaStream_t s) {
-  auto one = [&](bool staged, const void* w, size_t off, int64_t rows, int64_t cols, int64_t pitch, Matrix* m) {
-    if (!staged) {
-      *m = Matrix{const_cast<void*>(w), rows, cols, cols, 1, rows * cols};
-      return cudaSuccess;
-    }
-    *m = Matrix{ws + off, rows, cols, pitch, p.planes, rows * pitch};
-    return ff::stage(w, cols, rows, f->dtype, *m, s);
-  };
-  int rc;
-  if ((rc = cuda_rc(one(p.stage_c, wg, p.wg, f->hidden, f->width, p.pitch_c, &out->gate))) ||
-      (rc = cuda_rc(one(p.stage_c, wu, p.wu, f->hidden, f->width, p.pitch_c, &out->up))))
-    return rc;
-  return cuda_rc(one(p.stage_h, wd, p.wd, f->width_out, f->hidden, p.pitch_h, &out->down));
-}
+// Operands as the products read them: as they lie, or laid out anew by one kernel for all of a call's (the weights, then
+// the rows of each chunk).
+struct FfStage {
+  const trifast_ff* f;
+  const FfPlan* p;
+  char* ws;
+  ff::StageJob jobs[ff::kStageJobs];
+  int count = 0;
 
-// Rows [r0, r0 + rows) of x or dy.
-int ff_rows(const trifast_ff* f, const FfPlan& p, bool staged, const void* src, int64_t ld, int64_t r0, int64_t rows,
-            int64_t cols, int64_t pitch, void* at, Matrix* m, cudaStream_t s) {
-  const char* from = reinterpret_cast<const char*>(src) + (size_t)r0 * ld * elem(f->dtype);
-  if (!staged) {
-    *m = Matrix{const_cast<char*>(from), rows, cols, ld, 1, rows * ld};
-    return TRIFAST_OK;
+  Matrix matrix(bool staged, const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t pitch, int64_t padded, size_t off) {
+    if (!staged) return Matrix{const_cast<void*>(src), rows, cols, ld, 1, rows * ld};
+    const Matrix m{ws + off, rows, cols, pitch, p->planes, padded * pitch};
+    jobs[count++] = {src, ld, rows, m};
+    return m;
   }
-  *m = Matrix{at, rows, cols, pitch, p.planes, p.chunk * pitch};
-  return cuda_rc(ff::stage(from, ld, rows, f->dtype, *m, s));
-}
+  FfWeights weights(const void* wg, const void* wu, const void* wd) {
+    const trifast_ff& s = *f;
+    return {matrix(p->stage_c, wg, s.width, s.hidden, s.width, p->pitch_c, s.hidden, p->wg),
+            matrix(p->stage_c, wu, s.width, s.hidden, s.width, p->pitch_c, s.hidden, p->wu),
+            matrix(p->stage_h, wd, s.hidden, s.width_out, s.hidden, p->pitch_h, s.width_out, p->wd)};
+  }
+  // Rows [r0, r0 + rows) of x or dy.
+  Matrix rows(bool staged, const void* src, int64_t ld, int64_t r0, int64_t rows, int64_t cols, int64_t pitch, size_t off) {
+    return matrix(staged, reinterpret_cast<const char*>(src) + (size_t)r0 * ld * elem(f->dtype), ld, rows, cols, pitch, p->chunk, off);
+  }
+  int run(cudaStream_t s) {
+    const int n = count;
+    count = 0;
+    return cuda_rc(ff::stage(jobs, n, f->dtype, s));
+  }
+};
 
 ff::FusedArgs fused_args(const trifast_ff* f, const FfWeights& w, const Matrix& x, unsigned int* status) {
   ff::FusedArgs g = {};
@@ -278,12 +280,12 @@ int trifast_feed_forward(const trifast_ff* f, const void* x, const void* w_gate,
   if (p.few)
     return cuda_rc(ff::few_rows({x, w_gate, w_up, w_down, y, (float*)ws, f->ld_x, (int)f->rows, f->width, f->hidden, f->width_out,
                                  (int)p.pitch_h, f->dtype}, s));
-  FfWeights w;
-  if ((rc = ff_weights(f, p, ws, w_gate, w_up, w_down, &w, s))) return rc;
+  FfStage stage{f, &p, ws};
+  const FfWeights w = stage.weights(w_gate, w_up, w_down);
   for (int64_t r0 = 0; r0 < f->rows; r0 += p.chunk) {
     const int64_t rows = f->rows - r0 < p.chunk ? f->rows - r0 : p.chunk;
-    Matrix mx;
-    if ((rc = ff_rows(f, p, p.stage_x, x, f->ld_x, r0, rows, f->width, p.pitch_c, ws + p.x, &mx, s))) return rc;
+    const Matrix mx = stage.rows(p.stage_x, x, f->ld_x, r0, rows, f->width, p.pitch_c, p.x);
+    if ((rc = stage.run(s))) return rc;
     if (p.fused) {
       ff::FusedArgs g = fused_args(f, w, mx, status);
       g.what = ff::kForward;
@@ -334,15 +336,14 @@ int trifast_feed_forward_backward(const trifast_ff* f, const void* dy, const voi
     return rc;
   if (!dx && !weights) return TRIFAST_OK;
   char* ws = (char*)workspace;
-  FfWeights w;
-  if ((rc = ff_weights(f, p, ws, w_gate, w_up, w_down, &w, s))) return rc;
+  FfStage stage{f, &p, ws};
+  const FfWeights w = stage.weights(w_gate, w_up, w_down);
   float* partials = (float*)(ws + p.partials);
   for (int64_t r0 = 0; r0 < f->rows; r0 += p.chunk) {
     const int64_t rows = f->rows - r0 < p.chunk ? f->rows - r0 : p.chunk;
-    Matrix mx, mdy;
-    if ((rc = ff_rows(f, p, p.stage_x, x, f->ld_x, r0, rows, f->width, p.pitch_c, ws + p.x, &mx, s)) ||
-        (rc = ff_rows(f, p, p.stage_dy, dy, f->ld_dy, r0, rows, f->width_out, p.pitch_o, ws + p.dy, &mdy, s)))
-      return rc;
+    const Matrix mx = stage.rows(p.stage_x, x, f->ld_x, r0, rows, f->width, p.pitch_c, p.x);
+    const Matrix mdy = stage.rows(p.stage_dy, dy, f->ld_dy, r0, rows, f->width_out, p.pitch_o, p.dy);
+    if ((rc = stage.run(s))) return rc;
     if (p.fused) {
       ff::FusedArgs g = fused_args(f, w, mx, status);
       g.dy = mdy;

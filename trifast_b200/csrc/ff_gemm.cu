@@ -15,10 +15,10 @@
 // persistent, one per SM, the tiles of one row block next to one another.
 // Warps 0-7: epilogue (two warpgroups, each half of a tile's columns), 8: TMA, 9: MMA issuer.
 //
-// fp32: every value is the sum of three bf16 ones (ff_support.cu), and a product is the six
-// products of parts that are not below 2^-22 of it, the smallest first.  The accumulators in TMEM round towards
-// zero, so that a long sum drifts (5e-6 of the result over 384 MMAs): a sum ends after 256 of the contraction's
-// largest products, and the epilogue adds the sums up in fp32 registers, rounded to nearest.
+// fp32: every value is the sum of three bf16 ones (ff_support.cu), and a product is the six products of parts that are not
+// below 2^-22 of it.  A stage holds all three parts of both operands.  The accumulators in TMEM round towards zero, so
+// that a long sum drifts (5e-6 of the result over 384 MMAs): a sum takes one stage, the smallest products first, and
+// the epilogue adds the sums up in fp32 registers, rounded to nearest.
 //
 // What bounds it: the tiles' way from L2.  A 128 x 256 tile takes 48 KB per 64 of the contraction, for 512
 // cycles of the tensor pipe.
@@ -39,17 +39,18 @@ constexpr int kThreads = 320;
 constexpr int kSmemLimit = 232448;
 
 // Columns per B matrix (NT), accumulator columns, stages and staging of results by mode.
-template <int MODE, int NT, int CG>
+template <int PARTS, int MODE, int NT, int CG>
 struct Cfg {
   static constexpr int kAccCols = MODE == kGate || MODE == kHidden ? 2 * NT : NT;
   static constexpr int kBRows = MODE == kGate || MODE == kHidden ? 2 * NT : NT;   // largest of a stage, in all
-  static constexpr int kStageBytes = kTileA + kBRows / CG * kBK * 2;
+  static constexpr int kTileB = kBRows / CG * kBK * 2;
+  static constexpr int kStageBytes = PARTS * (kTileA + kTileB);   // all planes of A, then of B
   // result tiles of 128 rows x 64 columns
-  static constexpr int kOutTiles = MODE == kGate ? NT / 64 : MODE == kHidden ? 3 : MODE == kLinear ? 2 : 0;
+  static constexpr int kOutTiles = MODE == kGate ? NT / 64 : MODE == kHidden ? (PARTS == 3 ? 1 : 3) : MODE == kLinear && PARTS == 1 ? 2 : 0;
   static constexpr int kStages = (kSmemLimit - 2048 - kOutTiles * kTileA) / kStageBytes;
   static constexpr int kBufCols = kAccCols > 128 ? 256 : 128;    // TMEM columns between the two buffers
   static constexpr int smem_bytes() { return 1024 + 1024 + kStages * kStageBytes + kOutTiles * kTileA; }
-  static_assert(kAccCols <= 256 && kStages >= 3 && smem_bytes() <= kSmemLimit, "tile configuration");
+  static_assert(kAccCols <= 256 && kStages >= (PARTS == 3 ? 2 : 3) && smem_bytes() <= kSmemLimit, "tile configuration");
 };
 
 struct Params {
@@ -78,10 +79,8 @@ __device__ __forceinline__ uint32_t take_part(float& v0, float& v1) {
   return __byte_perm(a, b, 0x7632);
 }
 
-// Stages of the largest products that one sum in TMEM takes when PARTS is 3 (those of the smaller ones, five
-// times as many, go before the first).
-constexpr int kSumStages = 4;
-__device__ __forceinline__ int sums_of(int blocks) { return blocks <= kSumStages ? 1 : (blocks + kSumStages - 1) / kSumStages; }
+// Sums in TMEM that a contraction of so many stages takes when PARTS is 3 (an empty one takes one all the same).
+__device__ __forceinline__ int sums_of(int blocks) { return blocks < 1 ? 1 : blocks; }
 
 struct TileAt {
   int m0, n0;     // first row and column
@@ -112,7 +111,7 @@ __device__ __forceinline__ TileAt tile_at(const Params& p, int t, int rank) {
 // T: type of the operands; PARTS: planes of each (1, or 3 for fp32); OUT: type of kLinear's result.
 template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN, int CG>
 __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<MODE, NT, CG>;
+  using C = Cfg<PARTS, MODE, NT, CG>;
   constexpr int S = C::kStages;
   constexpr int FULL = 0, EMPTY = S, ACC_FULL = 2 * S, ACC_EMPTY = 2 * S + 2, NBARS = 2 * S + 4;
   static_assert(NBARS * 8 <= 240, "barrier area");
@@ -132,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
   // (the pair's first CTA counts what arrives, issues the MMAs and is told when results have been read)
   auto first_bar = [&](int i) -> uint32_t { return CG == 2 ? in_cta(bar(i), 0) : bar(i); };
   auto a_tile = [&](int s) -> uint32_t { return base + 1024 + s * C::kStageBytes; };
-  auto b_tile = [&](int s) -> uint32_t { return a_tile(s) + kTileA; };
+  auto b_tile = [&](int s) -> uint32_t { return a_tile(s) + PARTS * kTileA; };
   constexpr uint32_t out_off = 1024 + S * C::kStageBytes;
 
   after_previous();
@@ -193,8 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         int lo, hi;
         k_range(t, ph, lo, hi);
         const CUtensorMap* ma = &p.a[MODE == kWeight ? t.job : ph];
-        for (int q = 0; q < kPairs && ok; ++q) {
-          const int pa = kPairs == 1 ? 0 : plane_a(q), pb = kPairs == 1 ? 0 : plane_b(q);
+        {
           for (int kb = lo; kb < hi; ++kb, ++g) {
             const int s = g % S;
             if (g >= S) ok = mbar_wait(bar(EMPTY + s), ((g / S) - 1) & 1, abort_flag);
@@ -213,42 +211,31 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
                 else
                   tma_load_3d(dst, map, f, c0, c1, c2);
               };
-              // Wg and Wu: one each of the pair
-              auto load_gate_up = [&] {
-                if (CG == 2) {
-                  load(b_tile(s), &p.b[rank], kc, t.n0, pb);
-                } else {
-                  load(b_tile(s), &p.b[0], kc, t.n0, pb);
-                  load(b_tile(s) + NT * kBK * 2, &p.b[1], kc, t.n0, pb);
-                }
-              };
-              if constexpr (MODE == kHidden) {
-                expect(kTileA + (ph == 0 ? 1 : 2) * NT / CG * kBK * 2);
-                load(a_tile(s), ma, kc, t.m0, pa);
-                if (ph == 0) {
-#pragma unroll
-                  for (int i = 0; i < NT / CG / 64; ++i) load(b_tile(s) + i * 8192, &p.b[2], t.n0 + rank * (NT / CG) + 64 * i, kc, pb);
-                } else {
-                  load_gate_up();
-                }
-              } else {
+              if constexpr (MODE == kHidden)
+                expect(PARTS * (kTileA + (ph == 0 ? 1 : 2) * NT / CG * kBK * 2));
+              else
                 expect(C::kStageBytes);
+#pragma unroll
+              for (int q = 0; q < PARTS; ++q) {
+                const uint32_t at = a_tile(s) + q * kTileA, bt = b_tile(s) + q * C::kTileB;
+                const int n0 = t.n0 + rank * (NT / CG);   // this CTA's part of B's tile
                 if constexpr (kAMn) {
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) load(a_tile(s) + i * 8192, ma, t.m0 + 64 * i, kc, pa);
+                  for (int i = 0; i < 2; ++i) load(at + i * 8192, ma, t.m0 + 64 * i, kc, q);
                 } else {
-                  load(a_tile(s), ma, kc, t.m0, pa);
+                  load(at, ma, kc, t.m0, q);
                 }
-                if constexpr (MODE == kGate) {
-                  load_gate_up();
+                if (MODE == kGate || (MODE == kHidden && ph == 1)) {
+                  // Wg and Wu: one each of a pair
+                  load(bt, &p.b[rank], kc, t.n0, q);
+                  if (CG == 1) load(bt + NT * kBK * 2, &p.b[1], kc, t.n0, q);
                 } else {
-                  const CUtensorMap* mb = &p.b[MODE == kWeight ? t.job : ph];
-                  const int n0 = t.n0 + rank * (NT / CG);
-                  if constexpr (B_MN) {
+                  const CUtensorMap* mb = &p.b[MODE == kHidden ? 2 : MODE == kWeight ? t.job : ph];
+                  if constexpr (MODE == kHidden || B_MN) {
 #pragma unroll
-                    for (int i = 0; i < NT / CG / 64; ++i) load(b_tile(s) + i * 8192, mb, n0 + 64 * i, kc, pb);
+                    for (int i = 0; i < NT / CG / 64; ++i) load(bt + i * 8192, mb, n0 + 64 * i, kc, q);
                   } else {
-                    load(b_tile(s), mb, kc, n0, pb);
+                    load(bt, mb, kc, n0, q);
                   }
                 }
               }
@@ -293,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
       for (int ph = 0; ph < phases && ok; ++ph) {
         int lo, hi;
         k_range(t, ph, lo, hi);
-        const int steps = (hi - lo) * kPairs, small = (hi - lo) * (kPairs - 1);
+        const int steps = hi - lo;
         if (PARTS == 3 && ph > 0) {
           close_sum();
           open_sum();
@@ -305,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         // (kLinear's two products add up in one accumulator; kHidden's phases have their own)
         bool first = PARTS == 3 || MODE != kLinear || ph == 0;
         for (int i = 0; i < steps && ok; ++i, ++g) {
-          if (PARTS == 3 && i > small && (i - small) % kSumStages == 0) {
+          if (PARTS == 3 && i > 0) {
             close_sum();
             open_sum();
             if (!ok) break;
@@ -327,12 +314,16 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
             // 16 of the contraction: 32 bytes along a row, or 16 rows of an MN-major tile
             const uint32_t sa = kAMn ? 2048 >> 4 : 32 >> 4, sb = bmn ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk) {
-              const uint32_t add = (kk > 0 || !first) ? 1u : 0u;
-              if (CG == 2)
-                umma_ss_pair(d, ad + kk * sa, bd + kk * sb, idesc, add);
-              else
-                umma_ss(d, ad + kk * sa, bd + kk * sb, idesc, add);
+            for (int q = 0; q < kPairs; ++q) {
+              const uint32_t qa = PARTS == 3 ? plane_a(q) * (kTileA >> 4) : 0, qb = PARTS == 3 ? plane_b(q) * (C::kTileB >> 4) : 0;
+#pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk) {
+                const uint32_t add = (q > 0 || kk > 0 || !first) ? 1u : 0u;
+                if (CG == 2)
+                  umma_ss_pair(d, ad + kk * sa, bd + kk * sb, idesc, add);
+                else
+                  umma_ss(d, ad + qa + kk * sa, bd + qb + kk * sb, idesc, add);
+              }
             }
             commit(EMPTY + s);
           }
@@ -506,28 +497,45 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
             }
           }
           const int col = t.n0 + u0;
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
+          const bool inside = t.m0 < p.m[0] && col < p.n[0];
+          auto begin = [&] {
             if (leader) bulk_wait_read();
             group_sync(bar_id, kBarThreads);
+          };
+          auto put = [&](int tile, const uint32_t* u) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) *out_piece(tile, grp * 4 + c) = make_uint4(u[4 * c], u[4 * c + 1], u[4 * c + 2], u[4 * c + 3]);
+          };
+          auto end = [&] {
+            fence_async_smem();
+            group_sync(bar_id, kBarThreads);
+          };
+          if constexpr (PARTS == 1) {
+            begin();
+#pragma unroll
+            for (int o = 0; o < 3; ++o) put(o, packed[o]);
+            end();
+            if (leader && inside) {
+#pragma unroll
+              for (int o = 0; o < 3; ++o) tma_store_3d(&p.out[o], base + out_off + o * kTileA, col, t.m0, 0);
+              bulk_commit();
+            }
+          } else {
+            // (one result tile in shared memory: the operands' planes take the rest)
 #pragma unroll
             for (int o = 0; o < 3; ++o)
 #pragma unroll
-              for (int c = 0; c < 32; c += 8) {
-                if constexpr (PARTS == 3) {
+              for (int q = 0; q < PARTS; ++q) {
 #pragma unroll
-                  for (int e = 0; e < 8; e += 2) packed[o][(c + e) >> 1] = take_part(r[o][c + e], r[o][c + e + 1]);
+                for (int e = 0; e < 32; e += 2) packed[0][e >> 1] = take_part(r[o][e], r[o][e + 1]);
+                begin();
+                put(0, packed[0]);
+                end();
+                if (leader && inside) {
+                  tma_store_3d(&p.out[o], base + out_off, col, t.m0, q);
+                  bulk_commit();
                 }
-                const uint32_t* u = packed[o] + c / 2;
-                *out_piece(o, (grp * 32 + c) >> 3) = make_uint4(u[0], u[1], u[2], u[3]);
               }
-            fence_async_smem();
-            group_sync(bar_id, kBarThreads);
-            if (leader && t.m0 < p.m[0] && col < p.n[0]) {
-#pragma unroll
-              for (int o = 0; o < 3; ++o) tma_store_3d(&p.out[o], base + out_off + o * kTileA, col, t.m0, q);
-              bulk_commit();
-            }
           }
         }
       } else if constexpr (MODE == kLinear) {
@@ -658,7 +666,7 @@ bool weight_pairs(bool f32, std::initializer_list<int64_t> m) {
 
 template <typename T, int PARTS, typename OUT, int MODE, int NT, bool B_MN, int CG>
 cudaError_t launch_group(const GemmArgs& g, cudaStream_t stream) {
-  using C = Cfg<MODE, NT, CG>;
+  using C = Cfg<PARTS, MODE, NT, CG>;
   Params p = {};
   bool ok = true;
   int64_t tiles = 0;

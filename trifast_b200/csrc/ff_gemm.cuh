@@ -55,8 +55,14 @@ struct FewArgs {
 };
 cudaError_t few_rows(const FewArgs& a, cudaStream_t s);
 
-// dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of `dtype`)
-cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Matrix& dst, cudaStream_t s);
+// dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of the call's type, `ld` apart).
+struct StageJob {
+  const void* src;
+  int64_t ld, rows;
+  Matrix dst;
+};
+constexpr int kStageJobs = 5;
+cudaError_t stage(const StageJob* jobs, int count, int dtype, cudaStream_t s);
 // The sums over `splits` of partials[split * stride + i], in `dtype`: count[0] of them to dst[0], the next to dst[1], ...
 cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* const (&dst)[3], const int64_t (&count)[3], int dtype,
                          cudaStream_t s);

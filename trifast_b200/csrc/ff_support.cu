@@ -10,18 +10,28 @@ namespace trifast {
 namespace ff {
 namespace {
 
-// A matrix with rows of 16-byte pitch, and fp32 as three bf16 planes.  A value is cut, not rounded, to its
-// upper 8 significant bits, and what is left again: the three parts hold its 24 bits exactly and
-// have one sign.  A thread makes eight columns of a row; rows behind the last are zero.
+// Matrices with rows of 16-byte pitch, and fp32 as three bf16 planes.  A value is cut, not rounded, to its upper 8
+// significant bits, and what is left again: the three parts hold its 24 bits exactly and have one sign.  A thread makes
+// eight columns of a row; rows behind the last are zero.
+struct StageJobs {
+  StageJob job[kStageJobs];
+  int64_t end[kStageJobs];   // threads up to and with each
+  int count;
+};
 template <typename T>
-__global__ void stage_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, Matrix dst) {
+__global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ StageJobs jobs) {
   after_previous();
-  const int64_t per_row = dst.pitch / 8, total = dst.rows * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / per_row, c = (i % per_row) * 8;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < jobs.end[jobs.count - 1]; i += (int64_t)gridDim.x * blockDim.x) {
+    int j = 0;
+    while (i >= jobs.end[j]) ++j;
+    const StageJob& job = jobs.job[j];
+    const Matrix& dst = job.dst;
+    const int64_t at = i - (j ? jobs.end[j - 1] : 0), per_row = dst.pitch / 8;
+    const int64_t r = at / per_row, c = (at % per_row) * 8;
+    const T* src = reinterpret_cast<const T*>(job.src) + r * job.ld + c;
     T v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = r < rows && c + e < dst.cols ? src[r * ld + c + e] : from_f32<T>(0.f);
+    for (int e = 0; e < 8; ++e) v[e] = r < job.rows && c + e < dst.cols ? src[e] : from_f32<T>(0.f);
     uint16_t* out = reinterpret_cast<uint16_t*>(dst.p) + r * dst.pitch + c;
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
@@ -93,11 +103,16 @@ dim3 grid_for(int64_t threads) {
 
 }  // namespace
 
-cudaError_t stage(const void* src, int64_t ld, int64_t rows, int dtype, const Matrix& dst, cudaStream_t s) {
-  const int64_t threads = dst.rows * (dst.pitch / 8);
-  if (threads == 0) return cudaSuccess;
-  if (dtype == TRIFAST_F32) return launch_early(stage_kernel<float>, grid_for(threads), 256, 0, s, (const float*)src, ld, rows, dst);
-  return launch_early(stage_kernel<__half>, grid_for(threads), 256, 0, s, (const __half*)src, ld, rows, dst);
+cudaError_t stage(const StageJob* jobs, int count, int dtype, cudaStream_t s) {
+  StageJobs a = {};
+  for (int j = 0; j < count; ++j) {
+    a.job[a.count] = jobs[j];
+    a.end[a.count] = (a.count ? a.end[a.count - 1] : 0) + jobs[j].dst.rows * (jobs[j].dst.pitch / 8);
+    ++a.count;
+  }
+  if (count == 0) return cudaSuccess;
+  const dim3 g = grid_for(a.end[count - 1]);
+  return dtype == TRIFAST_F32 ? launch_early(stage_kernel<float>, g, 256, 0, s, a) : launch_early(stage_kernel<__half>, g, 256, 0, s, a);
 }
 
 template <typename T>
