@@ -74,7 +74,7 @@ def check(dy, x, wg, wu, wd, norm=True):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,c,h,o", [
     (1, 128, 512, 128),      # one token
-    (1, 1, 1, 1), (2, 3, 5, 7), (129, 8, 16, 8),
+    (1, 1, 1, 1), (2, 3, 5, 7), (129, 8, 16, 8), (129, 8, 520, 8), (65, 128, 1000, 100),
     (127, 64, 256, 64), (128, 128, 128, 128), (300, 128, 512, 128),
     (257, 100, 290, 100),    # rows that TMA cannot address
     (200, 130, 70, 66), (64, 72, 200, 264), (130, 264, 130, 40), (333, 256, 384, 128),
@@ -199,10 +199,11 @@ def test_same_bits_again():
         assert all(torch.equal(p, q) for p, q in zip(first, run(*case)))
 
 
-def test_rows_do_not_depend_on_their_neighbours():
+@pytest.mark.parametrize("hidden", [256, 576])
+def test_rows_do_not_depend_on_their_neighbours(hidden):
     """A row's result is the same in a batch of any size (of more than eight rows) and at any place of it."""
     from trifast_b200 import gated_feed_forward
-    _, x, *w = draw(400, 128, 256, 128, torch.bfloat16)
+    _, x, *w = draw(400, 128, hidden, 128, torch.bfloat16)
     y = gated_feed_forward(x, *w)
     for i in (0, 120, 128, 391):
         assert torch.equal(gated_feed_forward(x[i:i + 9], *w), y[i:i + 9])

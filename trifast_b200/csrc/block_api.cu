@@ -92,14 +92,18 @@ struct FfPlan {
   size_t wg, wu, wd, x, dy, h, da, db, partials, total;
 };
 
-// Rows from which on the fused kernels, which have one tile of 128 rows to a multiprocessor, are faster than
-// products that are split over the hidden units, too.
-constexpr int64_t kFusedRows = 148 * 64;
+// Where the fused kernels run, of those calls that they can take: they walk the hidden units one chunk of 64 after the
+// other, a tile of 128 rows to a multiprocessor, and are one kernel where the products are two or three.  Up to 512
+// units that is faster for any number of rows (512 rows, width 128, hidden 512: 11.4 against 12.7 us forward, 13.9 against
+// 15.7 for dX; hidden 256: 8.7 against 11.7 and 10.2 against 14.2), beyond, where there are tiles for half of the
+// multiprocessors.
+constexpr int kFusedHidden = 512;
+constexpr int64_t kFusedRows = 148 / 2 * 128;
 
 FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
   FfPlan p = {};
   const bool f32 = f->dtype == TRIFAST_F32;
-  p.fused = !f32 && f->width <= ff::kFusedWidth && f->width_out <= ff::kFusedWidth && f->rows >= kFusedRows;
+  p.fused = !f32 && f->width <= ff::kFusedWidth && f->width_out <= ff::kFusedWidth && (f->hidden <= kFusedHidden || f->rows >= kFusedRows);
   p.pitch_h = round_up(f->hidden, 8);
   p.few = !backward && f->rows <= ff::kFewRows;
   if (p.few) {

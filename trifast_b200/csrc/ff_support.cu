@@ -60,20 +60,25 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ Stag
   }
 }
 
-// The splits are added in order, in fp32; a thread makes four neighbours where all counts are multiples of four.
+// Eight warps of a block take an eighth of the splits each, in order, and their sums are added in order, all in fp32.  A
+// thread makes N neighbours: four where all counts are multiples of four.
 struct Results {
   void* dst[3];
   int64_t end[3];
 };
 template <typename T, int N>
 __global__ void __launch_bounds__(256) sum_partials_kernel(const float* __restrict__ partials, int splits, int64_t stride, Results r) {
+  __shared__ float sum[8][32 * N];
   after_previous();
-  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * N; i < r.end[2]; i += (int64_t)gridDim.x * blockDim.x * N) {
-    float s[N];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * N;
+  const int lo = splits * warp / 8, hi = splits * (warp + 1) / 8;
+  float s[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) s[e] = 0.f;
+  for (int e = 0; e < N; ++e) s[e] = 0.f;
+  if (i < r.end[2]) {
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
+    for (int k = lo; k < hi; ++k) {
       if constexpr (N == 4) {
         const float4 v = *reinterpret_cast<const float4*>(partials + k * stride + i);
         s[0] += v.x;
@@ -84,15 +89,23 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* __restri
         s[0] += partials[k * stride + i];
       }
     }
-    const int at = i < r.end[0] ? 0 : i < r.end[1] ? 1 : 2;
-    T* dst = reinterpret_cast<T*>(at == 0 ? r.dst[0] : at == 1 ? r.dst[1] : r.dst[2]) + (i - (at == 0 ? 0 : at == 1 ? r.end[0] : r.end[1]));
-    if constexpr (N == 4 && std::is_same<T, float>::value) {
-      *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[1], s[2], s[3]);
-    } else if constexpr (N == 4) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack2<T>(s[0], s[1]), tc::pack2<T>(s[2], s[3]));
-    } else {
-      *dst = from_f32<T>(s[0]);
-    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[warp][lane * N + e] = s[e];
+  __syncthreads();
+  if (warp != 0 || i >= r.end[2]) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] += sum[w][lane * N + e];
+  const int at = i < r.end[0] ? 0 : i < r.end[1] ? 1 : 2;
+  T* dst = reinterpret_cast<T*>(at == 0 ? r.dst[0] : at == 1 ? r.dst[1] : r.dst[2]) + (i - (at == 0 ? 0 : at == 1 ? r.end[0] : r.end[1]));
+  if constexpr (N == 4 && std::is_same<T, float>::value) {
+    *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[1], s[2], s[3]);
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack2<T>(s[0], s[1]), tc::pack2<T>(s[2], s[3]));
+  } else {
+    *dst = from_f32<T>(s[0]);
   }
 }
 
@@ -117,8 +130,8 @@ cudaError_t stage(const StageJob* jobs, int count, int dtype, cudaStream_t s) {
 
 template <typename T>
 cudaError_t sum_type(const float* partials, int splits, int64_t stride, const Results& r, bool four, cudaStream_t s) {
-  return four ? launch_early(sum_partials_kernel<T, 4>, grid_for(r.end[2] / 4), 256, 0, s, partials, splits, stride, r)
-              : launch_early(sum_partials_kernel<T, 1>, grid_for(r.end[2]), 256, 0, s, partials, splits, stride, r);
+  return four ? launch_early(sum_partials_kernel<T, 4>, dim3((unsigned)((r.end[2] + 127) / 128)), 256, 0, s, partials, splits, stride, r)
+              : launch_early(sum_partials_kernel<T, 1>, dim3((unsigned)((r.end[2] + 31) / 32)), 256, 0, s, partials, splits, stride, r);
 }
 
 cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* const (&dst)[3], const int64_t (&count)[3], int dtype,
