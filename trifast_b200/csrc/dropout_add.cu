@@ -26,11 +26,14 @@ __device__ __forceinline__ Words philox(uint64_t block, uint64_t offset, uint64_
   uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
-    const uint64_t p = (uint64_t)c0 * 0xD2511F53u, q = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(q >> 32) ^ c1 ^ k0;
-    c1 = (uint32_t)q;
-    c2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
-    c3 = (uint32_t)p;
+    const uint32_t ph = __umulhi(c0, 0xD2511F53u), qh = __umulhi(c2, 0xCD9E8D57u);
+    uint32_t pl, ql;
+    asm("mul.lo.u32 %0, %1, %2;" : "=r"(pl) : "r"(c0), "r"(0xD2511F53u));
+    asm("mul.lo.u32 %0, %1, %2;" : "=r"(ql) : "r"(c2), "r"(0xCD9E8D57u));
+    c0 = qh ^ c1 ^ k0;
+    c1 = ql;
+    c2 = ph ^ c3 ^ k1;
+    c3 = pl;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
@@ -173,6 +176,7 @@ __global__ void __launch_bounds__(256) dropout_own_kernel(DropoutArgs a) {
   const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
   for (int64_t i = i0; i < pieces; i += 2 * stride) {
     uint4 vx[2][N], vr[2][N];
+    Eight<T> mask[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       if (i + u * stride < pieces)
@@ -181,16 +185,19 @@ __global__ void __launch_bounds__(256) dropout_own_kernel(DropoutArgs a) {
           vx[u][k] = x[(i + u * stride) * N + k];
           if (RES) vr[u][k] = r[(i + u * stride) * N + k];
         }
+    // (four blocks of words side by side: a round is one chain of products)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (i + u * stride >= pieces) break;
       const uint64_t block = (uint64_t)(i + u * stride) * 2;
       const Words lo = philox(block, a.offset, key), hi = philox(block + 1, a.offset, key);
       const uint32_t w[8] = {lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]};
-      const Eight<T> mask = keep_mask<T>(w, a.threshold);
-#pragma unroll
-      for (int k = 0; k < N; ++k) y[(i + u * stride) * N + k] = apply<T, RES>(vx[u][k], vr[u][k], mask.v[k], a.scale);
+      mask[u] = keep_mask<T>(w, a.threshold);
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (i + u * stride < pieces)
+#pragma unroll
+        for (int k = 0; k < N; ++k) y[(i + u * stride) * N + k] = apply<T, RES>(vx[u][k], vr[u][k], mask[u].v[k], a.scale);
   }
   if (i0 < a.inner % 8) {
     const int64_t e = pieces * 8 + i0;
