@@ -144,7 +144,7 @@ FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
     // (the plan is the same on every device: 148 multiprocessors)
     const int64_t rows = f->rows < p.chunk ? f->rows : p.chunk;
     p.splits = p.fused ? ff::fused_weight_splits(rows, f->hidden, 148) : ff::weight_splits(m, n, rows, f32, 148);
-    p.partial_stride = round_up(f->hidden * (2 * (int64_t)f->width + f->width_out), 4);
+    p.partial_stride = 2 * f->hidden * ff::partial_pitch(f->width) + f->width_out * ff::partial_pitch(f->hidden);
     p.partials = take(true, p.splits * p.partial_stride * 4);
   }
   p.total = off;
@@ -406,8 +406,8 @@ int trifast_feed_forward_backward(const trifast_ff* f, const void* dy, const voi
     }
   }
   if (!weights) return TRIFAST_OK;
-  return cuda_rc(ff::sum_partials(partials, p.splits, p.partial_stride, {dw_gate, dw_up, dw_down}, {count_in, count_in, count_out},
-                                  f->dtype, s));
+  return cuda_rc(ff::sum_partials(partials, p.splits, p.partial_stride, {dw_gate, dw_up, dw_down}, {f->hidden, f->hidden, f->width_out},
+                                  {f->width, f->width, f->hidden}, f->dtype, s));
 }
 
 int trifast_dropout_add(const trifast_dropout* d, const int64_t* seed_device, const void* x, const void* residual, void* y,

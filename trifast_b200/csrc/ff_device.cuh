@@ -160,6 +160,22 @@ __device__ __forceinline__ void grad_units(const float* a, const float* b, const
   }
 }
 
+// 32 columns of a row of partial sums, of which `there` (a multiple of 4, or beyond 32) lie in the row.
+__device__ __forceinline__ void add_partials(float* dst, const float* v, int there, bool add) {
+  float4 u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    u[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    if (add && 4 * i < there) {
+      const float4 o = reinterpret_cast<const float4*>(dst)[i];
+      u[i] = make_float4(u[i].x + o.x, u[i].y + o.y, u[i].z + o.z, u[i].w + o.w);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (4 * i < there) reinterpret_cast<float4*>(dst)[i] = u[i];
+}
+
 // `box_cols` x `box_rows` tiles of a matrix
 inline bool map_of(CUtensorMap* map, bool bf16, const Matrix& m, int box_cols, int box_rows) {   // (128-byte swizzle; 64 for 32 columns)
   const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, (uint64_t)m.planes};

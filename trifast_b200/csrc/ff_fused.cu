@@ -683,25 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
     const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
     bool ok = true;
     float* part = p.partials + (int64_t)split * p.partial_stride;
-    const int64_t in = (int64_t)p.hidden * p.width;
-    auto put = [&](float* dst, const float* v, int cols, bool add) {   // 32 columns of a row, `cols` of them there
-      if (cols >= 32 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float4* q = reinterpret_cast<float4*>(dst + e);
-          float4 u = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          if (add) {
-            const float4 o = *q;
-            u = make_float4(u.x + o.x, u.y + o.y, u.z + o.z, u.w + o.w);
-          }
-          *q = u;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (e < cols) dst[e] = add ? dst[e] + v[e] : v[e];
-      }
-    };
+    const int pitch = (int)partial_pitch(p.width), pitch_d = (int)partial_pitch(p.hidden);
+    const int64_t in = (int64_t)p.hidden * pitch;
     // this group's half of the columns of the sums; unit: this thread's row of [dWg; dWu]
     auto flush = [&](bool add) {
       const int unit = chunk * kChunk + (row & 63);
@@ -711,13 +694,13 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
         float v[32];
         tmem_ld32(lanes + 320 + col, reinterpret_cast<uint32_t*>(v));
         tmem_wait_ld();
-        if (unit < p.hidden && col < p.width) put(part + (row >= 64 ? in : 0) + (int64_t)unit * p.width + col, v, p.width - col, add);
+        if (unit < p.hidden) add_partials(part + (row >= 64 ? in : 0) + (int64_t)unit * pitch + col, v, pitch - col, add);
       }
       float v[32];
       tmem_ld32(lanes + 448 + grp * 32, reinterpret_cast<uint32_t*>(v));
       tmem_wait_ld();
       const int col = chunk * kChunk + grp * 32;
-      if (row < p.width_out && col < p.hidden) put(part + 2 * in + (int64_t)row * p.hidden + col, v, p.hidden - col, add);
+      if (row < p.width_out) add_partials(part + 2 * in + (int64_t)row * pitch_d + col, v, pitch_d - col, add);
     };
     // 16-byte piece of this thread's row in staged tile `tile`
     auto piece = [&](int tile, int c16) -> uint4* {

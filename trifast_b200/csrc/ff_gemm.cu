@@ -599,8 +599,9 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         int64_t off = (int64_t)t.split * p.partial_stride;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          if (j < t.job) off += p.m[j] * p.n[j];
-        float* dst = p.partials + off + gr * n;
+          if (j < t.job) off += p.m[j] * partial_pitch(p.n[j]);
+        const int pitch = (int)partial_pitch(n);
+        float* dst = p.partials + off + gr * pitch;
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 32) {
           const int col = t.n0 + grp * kCols + c0;
@@ -611,24 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = 0.f;
           }
-          if (gr < p.m[t.job]) {
-            if (n % 4 == 0 && col + 32 <= n) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                float4* q = reinterpret_cast<float4*>(dst + col + e);
-                float4 u = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                if (p.add) {
-                  const float4 o = *q;
-                  u = make_float4(u.x + o.x, u.y + o.y, u.z + o.z, u.w + o.w);
-                }
-                *q = u;
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (col + e < n) dst[col + e] = p.add ? dst[col + e] + v[e] : v[e];
-            }
-          }
+          if (gr < p.m[t.job]) add_partials(dst + col, v, pitch - col, p.add);
         }
       }
     }

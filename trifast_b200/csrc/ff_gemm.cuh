@@ -33,13 +33,15 @@ struct GemmArgs {
   Matrix a[3], b[3]; // kGate: a0 = X, b = Wg, Wu.  kHidden: a0 = dY, a1 = X, b = Wg, Wu, Wd
   Matrix out[3];     // kGate: h.  kHidden: da, db, h.  kLinear: y, in the call's own type
   bool y_tma;        // TMA can write y
-  // kWeight: partial sums (splits, m0 * n0 + m1 * n1 + m2 * n2) fp32; added to what is there if `add`
+  // kWeight: partial sums, fp32, by split, product and row (of partial_pitch(n)); added to what is there if `add`
   float* partials;
   int64_t partial_stride;
   int splits;
   bool add;
   unsigned int* status;
 };
+// Row pitch of partial sums: whole 16-byte pieces.
+__host__ __device__ inline int64_t partial_pitch(int64_t n) { return (n + 3) / 4 * 4; }
 cudaError_t gemm(const GemmArgs& g, cudaStream_t s);
 // Row splits of a kWeight launch over `rows` rows whose products have m[i] x n[i] results.
 int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms);
@@ -63,9 +65,9 @@ struct StageJob {
 };
 constexpr int kStageJobs = 5;
 cudaError_t stage(const StageJob* jobs, int count, int dtype, cudaStream_t s);
-// The sums over `splits` of partials[split * stride + i], in `dtype`: count[0] of them to dst[0], the next to dst[1], ...
-cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* const (&dst)[3], const int64_t (&count)[3], int dtype,
-                         cudaStream_t s);
+// The sums over `splits` of three products' partial sums (rows[j] x cols[j] each), in `dtype`, to dst[0], dst[1] and dst[2].
+cudaError_t sum_partials(const float* partials, int splits, int64_t stride, void* const (&dst)[3], const int64_t (&rows)[3],
+                         const int64_t (&cols)[3], int dtype, cudaStream_t s);
 
 }  // namespace ff
 }  // namespace trifast

@@ -102,14 +102,16 @@ struct RowPieces {
   }
   // Whether some of the piece is not the row's: the first one's and the last one's lanes.
   __device__ __forceinline__ bool edge(int k) const { return SHIFT && (col(k) < 0 || col(k) + VEC > width); }
-  // `p`: the row's first element.  (Nothing is read behind the last row; before the first one lies nothing: its shift
-  // is 0.)
-  __device__ __forceinline__ void load(uint4* r, const T* p, int64_t row) const {
+  // Row `row` of `tensor`, zeros behind the last one.  (Nothing is read behind the tensor's end; before its beginning lies
+  // nothing of a piece: the first row's shift is 0.)
+  __device__ __forceinline__ void load(uint4* r, const void* tensor, int64_t ld, int64_t row) const {
+    const T* t = reinterpret_cast<const T*>(tensor);
+    const T *p = t + row * ld, *end = t + (rows - 1) * ld + width;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       r[k] = make_uint4(0, 0, 0, 0);
       if (row >= rows || !any(k)) continue;
-      if (SHIFT && row == rows - 1 && col(k) + VEC > width) {
+      if (SHIFT && p + col(k) + VEC > end) {
         T t[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) t[e] = has(k, e) ? p[col(k) + e] : from_f32<T>(0.f);
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_fwd_kernel(LayerNormAr
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = base + (r * kGroups + grp) * rows.step;
-      p.load(raw[r], reinterpret_cast<const T*>(a.x) + row * a.ld_x, row);
+      p.load(raw[r], a.x, a.ld_x, row);
     }
   };
   if (rows.first < a.rows) load(rows.first);
@@ -263,8 +265,8 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_bwd_kernel(LayerNormAr
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = base + (r * kGroups + grp) * rows.step;
-      p.load(raw_x[r], reinterpret_cast<const T*>(a.x) + row * a.ld_x, row);
-      p.load(raw_dy[r], reinterpret_cast<const T*>(a.dy) + row * a.ld_dy, row);
+      p.load(raw_x[r], a.x, a.ld_x, row);
+      p.load(raw_dy[r], a.dy, a.ld_dy, row);
     }
   };
   if (rows.first < a.rows) load(rows.first);
