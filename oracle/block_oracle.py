@@ -45,19 +45,21 @@ def feed_forward_grads(dy, x, w_gate, w_up, w_down):
     return (da @ wg + db @ wu).reshape(x.shape), da.T @ x2, db.T @ x2, dy2.T @ h
 
 
+def random_words_at(block, seed, offset=0):
+    """The four words of Philox-4x32-10 (Salmon et al., 2011) at counter (block, offset) under the key ``seed``."""
+    mask = 0xFFFFFFFF
+    c = [block & mask, (block >> 32) & mask, offset & mask, (offset >> 32) & mask]
+    k = [seed & mask, (seed >> 32) & mask]
+    for _ in range(10):
+        p, q = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(q >> 32) ^ c[1] ^ k[0], q & mask, (p >> 32) ^ c[3] ^ k[1], p & mask]
+        k = [(k[0] + 0x9E3779B9) & mask, (k[1] + 0xBB67AE85) & mask]
+    return c
+
+
 def random_words(count, seed, offset=0):
-    """Words 0 .. count - 1 of Philox-4x32-10 (Salmon et al., 2011) as a list of ints: word i is number i % 4
-    of counter (i // 4, offset) under the key ``seed``."""
-    mask, words = 0xFFFFFFFF, []
-    for block in range((count + 3) // 4):
-        c = [block & mask, (block >> 32) & mask, offset & mask, (offset >> 32) & mask]
-        k = [seed & mask, (seed >> 32) & mask]
-        for _ in range(10):
-            p, q = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
-            c = [(q >> 32) ^ c[1] ^ k[0], q & mask, (p >> 32) ^ c[3] ^ k[1], p & mask]
-            k = [(k[0] + 0x9E3779B9) & mask, (k[1] + 0xBB67AE85) & mask]
-        words += c
-    return words[:count]
+    """Words 0 .. count - 1 as a list of ints: word i is number i % 4 at counter (i // 4, offset)."""
+    return [w for block in range((count + 3) // 4) for w in random_words_at(block, seed, offset)][:count]
 
 
 def keep_mask(shape, p, seed, offset=0, shared_dim=None):

@@ -7,8 +7,10 @@ from oracle import block_oracle as oracle
 
 
 def test_generator_known_answers():
-    """The published vector of counter 0 under key 0; other counters, offsets and keys differ from it."""
+    """The published vectors: counter and key of zeros, and of ones."""
     assert oracle.random_words(4, 0) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = (1 << 64) - 1
+    assert oracle.random_words_at(ones, ones, ones) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
     a, b = oracle.random_words(8, 5, 9), oracle.random_words(8, 5, 10)
     assert a != b and a[:4] != a[4:]
     assert oracle.random_words(5, (1 << 64) - 1, 3) == oracle.random_words(8, -1, 3)[:5]

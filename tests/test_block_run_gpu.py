@@ -299,3 +299,81 @@ def test_workspace_of_the_feed_forward_does_not_grow_with_the_rows():
         size = [lib.trifast_feed_forward_backward_workspace_bytes(byref(_lib.FeedForward(r, 128, 128, 128, 512, 128, dtype)))
                 for r in (1 << 20, 1 << 24, 1 << 30)]
         assert all(0 < s < 320 << 20 for s in size)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^31 elements: the last rows are those of a call of their own."""
+    from trifast_b200 import dropout_add, gated_feed_forward, layer_norm
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free device memory")
+    for width, hidden in ((8, 8), (136, 8)):
+        rows = (1 << 31) // width + 1001
+        x = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+        x[-600:] = normal(600, width, seed=1, dtype=x.dtype)
+        w = normal(width, seed=2)
+        g, u, d = (normal(*s, seed=3 + i, dtype=x.dtype) for i, s in enumerate(((hidden, width), (hidden, width), (width, hidden))))
+        tail = x[-600:].clone()
+        assert torch.equal(layer_norm(x, w)[-600:], layer_norm(tail, w))
+        assert torch.equal(gated_feed_forward(x, g, u, d)[-600:], gated_feed_forward(tail, g, u, d))
+        dy = torch.zeros_like(x)
+        dy[-600:] = normal(600, width, seed=9, dtype=x.dtype)
+        grads = torch.ops.trifast_b200
+        for op, args in ((grads.layer_norm_grads, (w, 1e-5, True, False, False)), (grads.gated_feed_forward_grads, (g, u, d, True, False))):
+            a, b = op(dy, x, *args)[0], op(dy[-600:].clone(), tail, *args)[0]
+            assert torch.equal(a[-600:], b) and not a[:-600].any()
+            del a
+        y = dropout_add(x, dy, 0.5, 7, shared_dim=0)
+        assert torch.equal(y[-600:], dropout_add(tail, dy[-600:].clone(), 0.5, 7, shared_dim=0))
+        # every element its own: the last mask entries against those of the same counters at a small place
+        y = dropout_add(torch.ones_like(x), None, 0.5, 7)
+        blocks = [(x.numel() - 1) // 4 - i for i in range(3)]
+        for q in blocks:
+            want = torch.tensor([v >= 1 << 31 for v in block_oracle.random_words_at(q, 7)])
+            got = (y.view(-1)[4 * q:4 * q + 4] > 0).cpu()
+            assert torch.equal(got, want[:got.numel()])
+        del x, dy, y
+
+
+@pytest.mark.gpu
+def test_operators_pass_the_checks_of_tracing():
+    """Schema, fake kernels and autograd registration as torch.compile expects them."""
+    import trifast_b200  # noqa: F401
+    from torch.library import opcheck
+    ops = torch.ops.trifast_b200
+    t = lambda *s, i=0: normal(*s, seed=i, dtype=torch.float32).requires_grad_()
+    x, dy = t(2, 9, 16), normal(2, 9, 16, seed=7)
+    what = ("test_schema", "test_autograd_registration", "test_faketensor")
+    for op, args in ((ops.layer_norm, (x, t(16, i=1), t(16, i=2), 1e-5)), (ops.layer_norm, (x, None, None, 1e-5)),
+                     (ops.layer_norm_grads, (dy, x.detach(), normal(16, seed=1), 1e-5, True, True, False)),
+                     (ops.gated_feed_forward, (x, t(24, 16, i=1), t(24, 16, i=2), t(8, 24, i=3))),
+                     (ops.gated_feed_forward_grads, (normal(2, 9, 8, seed=4), x.detach(), *(normal(*s, seed=5) for s in ((24, 16), (24, 16), (8, 24))), True, True)),
+                     (ops.dropout_add, (x, t(2, 9, 16, i=3), 0.3, 5, 1, None, 1)),
+                     (ops.dropout_add, (x, None, 0.3, 0, 1, torch.tensor([4], device="cuda"), None))):
+        opcheck(op.default, args, test_utils=what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width,hidden", [(64, 64), (136, 64)])
+def test_after_a_kernel_that_gave_up(width, hidden):
+    """With the device's status set, a call raises; a kernel launched all the same writes nothing and ends."""
+    import ctypes as C
+
+    from trifast_b200 import _lib, gated_feed_forward
+    lib = _lib.load()
+    x = normal(300, width, seed=1, dtype=torch.bfloat16)
+    w = [normal(*s, seed=2, dtype=torch.bfloat16) for s in ((hidden, width), (hidden, width), (width, hidden))]
+    want = gated_feed_forward(x, *w)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(lib.trifast_debug_wait_probe(1000, stream), "trifast_debug_wait_probe")
+    y = torch.full_like(x, 7.0)
+    ff = _lib.FeedForward(300, width, width, width, hidden, width, 1)
+    size = lib.trifast_feed_forward_workspace_bytes(C.byref(ff))
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    args = [C.c_void_p(t.data_ptr()) for t in (x, *w, y, ws)]
+    _lib.check(lib.trifast_feed_forward(C.byref(ff), *args, size, stream), "trifast_feed_forward")
+    torch.cuda.synchronize()
+    assert torch.equal(y, torch.full_like(y, 7.0))
+    with pytest.raises(RuntimeError, match="gave up"):
+        gated_feed_forward(x, *w)
+    assert torch.equal(gated_feed_forward(x, *w), want)      # the status has been cleared

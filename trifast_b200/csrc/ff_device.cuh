@@ -21,6 +21,13 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
+// Whether an earlier kernel on this device has given up: the kernels then write nothing, and tell the host word again.
+__device__ __forceinline__ bool device_gave_up(unsigned int* status) {
+  const bool up = *reinterpret_cast<volatile unsigned int*>(status) != 0u;
+  if (up && blockIdx.x == 0 && threadIdx.x == 0) repeat_status(status);
+  return up;
+}
+
 // ------------------------------------------------------------------ pairs of CTAs (cta_group::2)
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_forward_kernel(const __grid
   const Smem sm = smem_of(smem_raw);
   volatile int* abort_flag = sm.abort_flag();
   after_previous();
-  const bool given_up = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
+  const bool given_up = device_gave_up(p.status);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), (i >= H_READY && i < H_READY + 3) || i == Y_FREE ? 8 : 1);
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
   const Smem sm = smem_of(smem_raw);
   volatile int* abort_flag = sm.abort_flag();
   after_previous();
-  const bool given_up = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
+  const bool given_up = device_gave_up(p.status);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), i == DX_FREE ? 8 : (i >= P_READY && i < P_READY + 2) ? 16 : 1);
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
   const Smem sm = smem_of(smem_raw);
   volatile int* abort_flag = sm.abort_flag();
   after_previous();
-  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+  if (device_gave_up(p.status)) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NBARS; ++i) mbar_init(sm.bar(i), i == DH_FREE || i == STG_READY || i == ACC_FREE ? 8 : 1);

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
   constexpr uint32_t out_off = 1024 + S * C::kStageBytes;
 
   after_previous();
-  const bool given_up = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
+  const bool given_up = device_gave_up(p.status);
   if (CG == 1 && given_up) return;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
