@@ -107,7 +107,8 @@ FfPlan plan_ff(const trifast_ff* f, bool backward, bool weights) {
   p.pitch_h = round_up(f->hidden, 8);
   p.few = !backward && f->rows <= ff::kFewRows;
   if (p.few) {
-    p.total = (size_t)round_up(f->rows * p.pitch_h * 4, 256);
+    if (!ff::few_rows_in_cluster(f->rows, f->width, f->hidden, f->width_out, (int)elem(f->dtype)))
+      p.total = (size_t)round_up(f->rows * p.pitch_h * 4, 256);
     return p;
   }
   p.planes = f32 ? 3 : 1;

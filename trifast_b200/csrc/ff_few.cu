@@ -1,13 +1,14 @@
 // The feed-forward block's forward pass for a few rows (a token or so at a time): both products on the CUDA cores, a
 // warp to a hidden unit and then to a result, which read every weight once.  Hidden values are fp32.
 //
-// What bounds it: the launches, and the latency of one read of the weights (width 128, hidden 512, one row: 11.0 us a
-// call on the tensor-core kernels, whose tiles are 128 rows and whose 2 x 4 tiles walk the contraction alone).
+// What bounds it: the launches, and the latency of one read of the weights.  Small blocks (kClusterBytes of weights) are
+// one kernel, a cluster of eight CTAs whose warps write their hidden values into the shared memory of all eight; larger
+// ones two kernels over all multiprocessors.  (Width 128, hidden 512, one row: 11.0 us a call on the tensor-core
+// kernels, whose tiles are 128 rows, 9.5 as two kernels.)
 
 #include <type_traits>
 
-#include "ff_gemm.cuh"
-#include "tc_common.cuh"
+#include "ff_device.cuh"
 
 namespace trifast {
 namespace ff {
@@ -46,19 +47,16 @@ __device__ __forceinline__ void warp_sum(float* v) {
     for (int r = 0; r < R; ++r) v[r] += __shfl_xor_sync(0xffffffffu, v[r], m);
 }
 
+// silu(x wg^T) * (x wu^T) of one hidden unit: in lane r that of row r
 template <typename T, int R, int N>
-__global__ void __launch_bounds__(32 * kWarps) few_hidden_kernel(const T* __restrict__ x, int64_t ld, int rows, const T* __restrict__ wg,
-                                                                 const T* __restrict__ wu, float* __restrict__ h, int width, int hidden,
-                                                                 int pitch) {
-  after_previous();
-  const int unit = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (unit >= hidden) return;
+__device__ __forceinline__ float unit_value(const T* __restrict__ x, int64_t ld, int rows, const T* __restrict__ wg, const T* __restrict__ wu,
+                                            int width, int lane) {
   float a[R] = {}, b[R] = {};
 #pragma unroll 2
   for (int c = lane * N; c < width; c += 32 * N) {
     float g[N], u[N];
-    read<T, N>(wg + (int64_t)unit * width + c, g);
-    read<T, N>(wu + (int64_t)unit * width + c, u);
+    read<T, N>(wg + c, g);
+    read<T, N>(wu + c, u);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float v[N];
@@ -72,22 +70,21 @@ __global__ void __launch_bounds__(32 * kWarps) few_hidden_kernel(const T* __rest
   }
   warp_sum<R>(a);
   warp_sum<R>(b);
+  float h = 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (lane == r && r < rows) h[r * pitch + unit] = a[r] / (1.f + expf(-a[r])) * b[r];
+    if (lane == r) h = a[r] / (1.f + expf(-a[r])) * b[r];
+  return h;
 }
 
+// One result: in lane r that of row r (h: rows `pitch` apart)
 template <typename T, int R, int N>
-__global__ void __launch_bounds__(32 * kWarps) few_result_kernel(const float* __restrict__ h, int rows, const T* __restrict__ wd, T* __restrict__ y,
-                                                                 int hidden, int pitch, int width_out) {
-  after_previous();
-  const int o = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (o >= width_out) return;
+__device__ __forceinline__ float result_value(const float* h, int rows, const T* __restrict__ wd, int hidden, int pitch, int lane) {
   float s[R] = {};
 #pragma unroll 2
   for (int c = lane * N; c < hidden; c += 32 * N) {
     float w[N];
-    read<T, N>(wd + (int64_t)o * hidden + c, w);
+    read<T, N>(wd + c, w);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float v[N];
@@ -97,22 +94,70 @@ __global__ void __launch_bounds__(32 * kWarps) few_result_kernel(const float* __
     }
   }
   warp_sum<R>(s);
+  float y = 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (lane == r && r < rows) y[(int64_t)r * width_out + o] = from_f32<T>(s[r]);
+    if (lane == r) y = s[r];
+  return y;
+}
+
+template <typename T, int R, int N>
+__global__ void __launch_bounds__(32 * kWarps) few_hidden_kernel(FewArgs p) {
+  after_previous();
+  const int unit = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (unit >= p.hidden) return;
+  const float h = unit_value<T, R, N>((const T*)p.x, p.ld, p.rows, (const T*)p.wg + (int64_t)unit * p.width, (const T*)p.wu + (int64_t)unit * p.width,
+                                      p.width, lane);
+  if (lane < p.rows) p.h[lane * p.pitch + unit] = h;
+}
+
+template <typename T, int R, int N>
+__global__ void __launch_bounds__(32 * kWarps) few_result_kernel(FewArgs p) {
+  after_previous();
+  const int o = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (o >= p.width_out) return;
+  const float y = result_value<T, R, N>(p.h, p.rows, (const T*)p.wd + (int64_t)o * p.hidden, p.hidden, p.pitch, lane);
+  if (lane < p.rows) ((T*)p.y)[(int64_t)lane * p.width_out + o] = from_f32<T>(y);
+}
+
+// Both, by a cluster.  N, M: neighbours read at a time along the width and along the hidden units.
+constexpr int kClusterCtas = 8, kClusterThreads = 1024, kClusterWarps = kClusterCtas * kClusterThreads / 32;
+template <typename T, int R, int N, int M>
+__global__ void __launch_bounds__(kClusterThreads) few_cluster_kernel(FewArgs p) {
+  extern __shared__ __align__(16) float few_h[];   // (rows, pitch)
+  after_previous();
+  const int rank = (int)cluster_rank(), warp = rank * (kClusterThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t own = tc::smem_u32(few_h);
+  cluster_sync();   // (all CTAs are there to be written to)
+  for (int unit = warp; unit < p.hidden; unit += kClusterWarps) {
+    const float h = unit_value<T, R, N>((const T*)p.x, p.ld, p.rows, (const T*)p.wg + (int64_t)unit * p.width,
+                                        (const T*)p.wu + (int64_t)unit * p.width, p.width, lane);
+    if (lane < p.rows) {
+#pragma unroll
+      for (int c = 0; c < kClusterCtas; ++c)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(own + 4u * (lane * p.pitch + unit), c)), "f"(h) : "memory");
+    }
+  }
+  cluster_sync();
+  for (int o = warp; o < p.width_out; o += kClusterWarps) {
+    const float y = result_value<T, R, M>(few_h, p.rows, (const T*)p.wd + (int64_t)o * p.hidden, p.hidden, p.pitch, lane);
+    if (lane < p.rows) ((T*)p.y)[(int64_t)lane * p.width_out + o] = from_f32<T>(y);
+  }
 }
 
 template <typename T, int R>
 cudaError_t launch(const FewArgs& a, cudaStream_t s) {
   constexpr int N = 16 / sizeof(T);
-  const int blocks = (a.hidden + kWarps - 1) / kWarps, outs = (a.width_out + kWarps - 1) / kWarps;
-  const T *x = (const T*)a.x, *wg = (const T*)a.wg, *wu = (const T*)a.wu, *wd = (const T*)a.wd;
-  const bool whole = a.width % N == 0 && (a.rows == 1 || a.ld % N == 0);
-  cudaError_t e = launch_early(whole ? few_hidden_kernel<T, R, N> : few_hidden_kernel<T, R, 1>, dim3(blocks), 32 * kWarps, 0, s, x, a.ld, a.rows,
-                               wg, wu, a.h, a.width, a.hidden, a.pitch);
+  const bool in = a.width % N == 0 && (a.rows == 1 || a.ld % N == 0), out = a.hidden % N == 0;
+  if (few_rows_in_cluster(a.rows, a.width, a.hidden, a.width_out, sizeof(T))) {
+    const auto kern = in && out ? few_cluster_kernel<T, R, N, N> : in ? few_cluster_kernel<T, R, N, 1> : out ? few_cluster_kernel<T, R, 1, N>
+                                                                                                        : few_cluster_kernel<T, R, 1, 1>;
+    return launch_clusters(kern, dim3(kClusterCtas), kClusterThreads, (size_t)a.rows * a.pitch * sizeof(float), s, kClusterCtas, a);
+  }
+  const int units = (a.hidden + kWarps - 1) / kWarps, results = (a.width_out + kWarps - 1) / kWarps;
+  const cudaError_t e = launch_early(in ? few_hidden_kernel<T, R, N> : few_hidden_kernel<T, R, 1>, dim3(units), 32 * kWarps, 0, s, a);
   if (e != cudaSuccess) return e;
-  return launch_early(a.hidden % N == 0 ? few_result_kernel<T, R, N> : few_result_kernel<T, R, 1>, dim3(outs), 32 * kWarps, 0, s,
-                      (const float*)a.h, a.rows, wd, (T*)a.y, a.hidden, a.pitch, a.width_out);
+  return launch_early(out ? few_result_kernel<T, R, N> : few_result_kernel<T, R, 1>, dim3(results), 32 * kWarps, 0, s, a);
 }
 
 template <typename T>
@@ -121,6 +166,12 @@ cudaError_t launch_rows(const FewArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+// One cluster reads at most a megabyte of weights (eight multiprocessors would take longer over more), and its hidden
+// values fit the shared memory that needs no opt-in.
+bool few_rows_in_cluster(int64_t rows, int64_t width, int64_t hidden, int64_t width_out, int elem) {
+  return hidden * (2 * width + width_out) * elem <= 1 << 20 && rows * ((hidden + 7) / 8 * 8) * (int64_t)sizeof(float) <= 40 << 10;
+}
 
 cudaError_t few_rows(const FewArgs& a, cudaStream_t s) {
   switch (a.dtype) {

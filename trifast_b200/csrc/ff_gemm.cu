@@ -541,22 +541,24 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
       } else if constexpr (MODE == kLinear) {
         const int64_t gr = (int64_t)t.m0 + row;
         OUT* yr = reinterpret_cast<OUT*>(p.y) + gr * p.ldy;
+        constexpr int kStep = kCols < 64 ? kCols : 64;
+        static_assert(MODE != kLinear || PARTS == 3 || kStep == 64, "result tiles are 64 columns");
 #pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += 64) {
+        for (int c0 = 0; c0 < kCols; c0 += kStep) {
           const int col = t.n0 + grp * kCols + c0;
-          float v[64];
-          columns(0, c0, v);
-          columns(0, c0 + 32, v + 32);
-          loaded(c0 + 64 == kCols);
+          float v[kStep];
+#pragma unroll
+          for (int c = 0; c < kStep; c += 32) columns(0, c0 + c, v + c);
+          loaded(c0 + kStep == kCols);
           if constexpr (std::is_same<OUT, float>::value) {
             if (gr < p.m[0]) {
-              if (p.ldy % 4 == 0 && col + 64 <= p.n[0] && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
+              if (p.ldy % 4 == 0 && col + kStep <= p.n[0] && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
 #pragma unroll
-                for (int e = 0; e < 64; e += 4)
+                for (int e = 0; e < kStep; e += 4)
                   *reinterpret_cast<float4*>(yr + col + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
               } else {
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
+                for (int e = 0; e < kStep; ++e)
                   if (col + e < p.n[0]) yr[col + e] = v[e];
               }
             }
@@ -728,7 +730,13 @@ cudaError_t dispatch(const GemmArgs& g, cudaStream_t s) {
     case kGate: return launch<T, PARTS, OUT, kGate, kWide / 2, false>(g, s);
     case kHidden: return launch<T, PARTS, OUT, kHidden, PARTS == 3 ? 64 : 128, false>(g, s);
     case kLinear: {
-      const bool wide = wide_tiles(PARTS == 3, {g.b_mn ? g.b[0].cols : g.b[0].rows});
+      const int64_t n = g.b_mn ? g.b[0].cols : g.b[0].rows;
+      if constexpr (PARTS == 3) {
+        // 64 columns where tiles of 128 leave multiprocessors without one (5041 rows, width 100, fp32: dX 22.2 us)
+        if (tiles_of(g.a[0].rows, 128) * tiles_of(n, 128) < sm_count())
+          return g.b_mn ? launch<T, PARTS, OUT, kLinear, 64, true>(g, s) : launch<T, PARTS, OUT, kLinear, 64, false>(g, s);
+      }
+      const bool wide = wide_tiles(PARTS == 3, {n});
       if (g.b_mn) return wide ? launch<T, PARTS, OUT, kLinear, kWide, true>(g, s) : launch<T, PARTS, OUT, kLinear, 128, true>(g, s);
       return wide ? launch<T, PARTS, OUT, kLinear, kWide, false>(g, s) : launch<T, PARTS, OUT, kLinear, 128, false>(g, s);
     }

@@ -51,11 +51,12 @@ constexpr int kFewRows = 8;
 struct FewArgs {
   const void *x, *wg, *wu, *wd;
   void* y;
-  float* h;
+  float* h;        // not used by a cluster
   int64_t ld;
   int rows, width, hidden, width_out, pitch, dtype;
 };
 cudaError_t few_rows(const FewArgs& a, cudaStream_t s);
+bool few_rows_in_cluster(int64_t rows, int64_t width, int64_t hidden, int64_t width_out, int elem);   // (needs no h)
 
 // dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of the call's type, `ld` apart).
 struct StageJob {
