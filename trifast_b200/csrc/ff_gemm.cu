@@ -5,23 +5,25 @@
 //     dX = da Wg + db Wu,  dWg = da^T X,  dWu = db^T X,  dWd = dY^T h
 // on the tensor cores, as one kernel with four epilogues (Mode in ff_gemm.cuh).
 //
-// A tile has 128 rows and up to 256 fp32 columns in TMEM, twice, so that the epilogue of one tile runs
-// under the MMAs of the next.  (kHidden has 128 units a tile: a and b once, 256 columns, dH twice, so that the next dH
-// runs under the epilogue: with 64 units, all of them twice, X and dY came from L2 twice as often, which bounds this
-// kernel: 72 us for 8192 rows, width 512, hidden 2048.)  Where there is more than one row tile, two CTAs share an MMA (CG = 2): each has its 128
-// rows of A and of the result, and half of B's tile, which the tensor cores of both read.  Operands come in blocks of 64 along the contraction, through a ring of
-// stages that TMA fills (128-byte swizzle).  Both majors are read as they lie: where the contraction
-// runs along a matrix's rows the tile is an MN-major operand of 64-element columns.  CTAs are
-// persistent, one per SM, the tiles of one row block next to one another.
-// Warps 0-7: epilogue (two warpgroups, each half of a tile's columns), 8: TMA, 9: MMA issuer.
+// A tile has 128 rows and up to 256 fp32 columns in TMEM, twice, so that the epilogue of one tile runs under the MMAs of
+// the next.  Where there is more than one row tile, two CTAs share an MMA (CG = 2): each has its 128 rows of A and of
+// the result, and half of B's tile, which the tensor cores of both read.  kHidden has 128 units a tile: a and b once, 256
+// columns, dH twice, so that the next dH runs under the epilogue (64 units, all of them twice, fetched X and dY twice as
+// often: 72 us of 58 for 8192 rows, width 512, hidden 2048).
+//
+// Operands come in blocks of 64 along the contraction, through a ring of stages that TMA fills (128-byte swizzle).
+// Both majors are read as they lie: where the contraction runs along a matrix's rows the tile is an MN-major operand of
+// 64-element columns.  CTAs are persistent, one per SM, the tiles of one row block next to one another.
+// Warps 0-7: epilogue (two warpgroups, each half of a tile's columns), 8: TMA, 9: MMA issuer (of the pair's first CTA).
 //
 // fp32: every value is the sum of three bf16 ones (ff_support.cu), and a product is the six products of parts that are not
 // below 2^-22 of it.  A stage holds all three parts of both operands.  The accumulators in TMEM round towards zero, so
 // that a long sum drifts (5e-6 of the result over 384 MMAs): a sum takes one stage, the smallest products first, and
 // the epilogue adds the sums up in fp32 registers, rounded to nearest.
 //
-// What bounds it: the tiles' way from L2.  A 128 x 256 tile takes 48 KB per 64 of the contraction, for 512
-// cycles of the tensor pipe.
+// What bounds it: the tiles' way from L2.  A pair's 256 x 256 tile takes 32 KB a CTA per 64 of the contraction, which the
+// tensor pipe works on for 512 cycles: 64 bytes a cycle, of which about 42 arrive (10.7 TB/s on all SMs).  65,536 rows of
+// 512, hidden 1024, bf16: 110 us for the gate, 56 for the result, 1.25 PFLOP/s.
 
 #include <initializer_list>
 #include <type_traits>
@@ -192,56 +194,54 @@ __global__ void __launch_bounds__(kThreads, 1) ff_gemm_kernel(const __grid_const
         int lo, hi;
         k_range(t, ph, lo, hi);
         const CUtensorMap* ma = &p.a[MODE == kWeight ? t.job : ph];
-        {
-          for (int kb = lo; kb < hi; ++kb, ++g) {
-            const int s = g % S;
-            if (g >= S) ok = mbar_wait(bar(EMPTY + s), ((g / S) - 1) & 1, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (elect_one()) {
-              const uint32_t f = first_bar(FULL + s);
-              const int kc = kb * kBK;
-              // (the first CTA's arrival, with the bytes of both)
-              auto expect = [&](int bytes) {
-                if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), CG * bytes);
-              };
-              auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
-                if (CG == 2)
-                  tma_load_3d_pair(dst, map, f, c0, c1, c2);
-                else
-                  tma_load_3d(dst, map, f, c0, c1, c2);
-              };
-              if constexpr (MODE == kHidden)
-                expect(PARTS * (kTileA + (ph == 0 ? 1 : 2) * NT / CG * kBK * 2));
+        for (int kb = lo; kb < hi; ++kb, ++g) {
+          const int s = g % S;
+          if (g >= S) ok = mbar_wait(bar(EMPTY + s), ((g / S) - 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (elect_one()) {
+            const uint32_t f = first_bar(FULL + s);
+            const int kc = kb * kBK;
+            // (the first CTA's arrival, with the bytes of both)
+            auto expect = [&](int bytes) {
+              if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), CG * bytes);
+            };
+            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+              if (CG == 2)
+                tma_load_3d_pair(dst, map, f, c0, c1, c2);
               else
-                expect(C::kStageBytes);
+                tma_load_3d(dst, map, f, c0, c1, c2);
+            };
+            if constexpr (MODE == kHidden)
+              expect(PARTS * (kTileA + (ph == 0 ? 1 : 2) * NT / CG * kBK * 2));
+            else
+              expect(C::kStageBytes);
 #pragma unroll
-              for (int q = 0; q < PARTS; ++q) {
-                const uint32_t at = a_tile(s) + q * kTileA, bt = b_tile(s) + q * C::kTileB;
-                const int n0 = t.n0 + rank * (NT / CG);   // this CTA's part of B's tile
-                if constexpr (kAMn) {
+            for (int q = 0; q < PARTS; ++q) {
+              const uint32_t at = a_tile(s) + q * kTileA, bt = b_tile(s) + q * C::kTileB;
+              const int n0 = t.n0 + rank * (NT / CG);   // this CTA's part of B's tile
+              if constexpr (kAMn) {
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) load(at + i * 8192, ma, t.m0 + 64 * i, kc, q);
+                for (int i = 0; i < 2; ++i) load(at + i * 8192, ma, t.m0 + 64 * i, kc, q);
+              } else {
+                load(at, ma, kc, t.m0, q);
+              }
+              if (MODE == kGate || (MODE == kHidden && ph == 1)) {
+                // Wg and Wu: one each of a pair
+                load(bt, &p.b[rank], kc, t.n0, q);
+                if (CG == 1) load(bt + NT * kBK * 2, &p.b[1], kc, t.n0, q);
+              } else {
+                const CUtensorMap* mb = &p.b[MODE == kHidden ? 2 : MODE == kWeight ? t.job : ph];
+                if constexpr (MODE == kHidden || B_MN) {
+#pragma unroll
+                  for (int i = 0; i < NT / CG / 64; ++i) load(bt + i * 8192, mb, n0 + 64 * i, kc, q);
                 } else {
-                  load(at, ma, kc, t.m0, q);
-                }
-                if (MODE == kGate || (MODE == kHidden && ph == 1)) {
-                  // Wg and Wu: one each of a pair
-                  load(bt, &p.b[rank], kc, t.n0, q);
-                  if (CG == 1) load(bt + NT * kBK * 2, &p.b[1], kc, t.n0, q);
-                } else {
-                  const CUtensorMap* mb = &p.b[MODE == kHidden ? 2 : MODE == kWeight ? t.job : ph];
-                  if constexpr (MODE == kHidden || B_MN) {
-#pragma unroll
-                    for (int i = 0; i < NT / CG / 64; ++i) load(bt + i * 8192, mb, n0 + 64 * i, kc, q);
-                  } else {
-                    load(bt, mb, kc, n0, q);
-                  }
+                  load(bt, mb, kc, n0, q);
                 }
               }
             }
-            __syncwarp();
           }
+          __syncwarp();
         }
       }
     }
