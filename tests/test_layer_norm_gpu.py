@@ -115,6 +115,42 @@ def test_nonfinite_rows_stay_in_their_rows():
     assert torch.equal(y[keep], clean[keep])
 
 
+
+# widths of each way of sharing a row among threads, whose rows begin and end inside 16-byte pieces
+ODD_WIDTHS = [1, 2, 3, 5, 7, 9, 25, 27, 33, 59, 65, 91, 101, 129, 249, 251, 257, 301, 505, 507, 777, 1023, 1273, 1275, 1999, 2553, 2555,
+              2901, 4089, 4091, 5001, 5113, 5115, 8001, 8185]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", ODD_WIDTHS)
+def test_rows_inside_pieces(width, dtype):
+    """Every class of rows, more than one turn of a block, a mean of many deviations."""
+    rows = max(21, min(5003, 400_000 // width))
+    x, dy = normal(rows, width, seed=1, dtype=dtype), normal(rows, width, seed=2, dtype=dtype)
+    x[::3] += 30.0
+    check(x, (1 + 0.3 * normal(width, seed=3)).to(dtype), (0.3 * normal(width, seed=4)).to(dtype), dy)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [3, 9, 65, 301, 1023, 1999, 2901, 4091, 5001, 8001])
+def test_neighbours_of_rows_inside_pieces(width, dtype):
+    """What lies in a row's first and last piece beside it (rows that are not finite, here) is not seen."""
+    from trifast_b200 import layer_norm
+    x, dy = normal(24, width, seed=1, dtype=dtype), normal(24, width, seed=2, dtype=dtype)
+
+    def run(x, dy):
+        leaf = x.clone().requires_grad_()
+        y = layer_norm(leaf)
+        return y.detach(), torch.autograd.grad(y, leaf, dy)[0]
+    clean = run(x, dy)
+    bad, bad_dy = x.clone(), dy.clone()
+    bad[::2] = float("nan")
+    bad_dy[::2] = float("inf")
+    got = run(bad, bad_dy)
+    for c, g in zip(clean, got):
+        assert torch.equal(c[1::2], g[1::2]) and g[::2].isnan().all()
+
+
 def test_only_what_is_asked_for():
     from trifast_b200 import layer_norm
     x, w, b = normal(50, 96, seed=1), normal(96, seed=2), normal(96, seed=3)

@@ -11,10 +11,11 @@
 //
 // Rows whose bytes are no multiple of 16 (SHIFT) are read in the 16-byte pieces that they lie in all the same: rows of
 // one class modulo 8 (fp32: 4) begin at the same place of a piece, and a block takes rows of one class, so that its
-// threads keep their columns.  What a piece holds of other rows is set to zero.
+// threads keep their columns.  What a piece holds of other rows is replaced.
 //
-// What bounds it: memory (1,048,576 x 128 bf16: 87 us forward, 135 backward, 6.2 and 6.0 TB/s).  Rows beyond 8192 elements
-// (kMaxRow) are walked in passes instead.
+// What bounds it: memory (1,048,576 x 128 bf16: 87 us forward, 135 backward, 6.2 and 6.0 TB/s); with SHIFT the instructions
+// of its edges and the registers of their masks (65,536 x 1999 bf16: 110 and 222 us, 2000: 94 and 161).  Rows beyond 8192
+// elements (kMaxRow) are walked in passes instead.
 
 #include <type_traits>
 
@@ -63,7 +64,15 @@ __device__ __forceinline__ float affine_at(const void* p, int dtype, int i) {
 }
 
 // Sums over the TPR threads of a row, N at a time.  `buf`: shared memory of each call site's own, two
-// call sites at least in a loop (a thread that is a call behind still reads the other's).
+// call sites at least in a loop (a thread that is a call behind still reads the other's); no_sums() before the first.
+template <int TPR, int N>
+__device__ __forceinline__ void no_sums(float (*buf)[N][32]) {   // of the warps that the block has not
+  if constexpr (TPR > 32)
+    for (int i = threadIdx.x; i < 2 * N * 32; i += blockDim.x) {
+      const int w = i % 32;
+      if (w * 32 >= (int)blockDim.x) buf[i / 32 / N][i / 32 % N][w] = 0.f;
+    }
+}
 template <int TPR, int N>
 __device__ __forceinline__ void row_sums(float* v, float (*buf)[32]) {
 #pragma unroll
@@ -87,32 +96,59 @@ __device__ __forceinline__ void row_sums(float* v, float (*buf)[32]) {
   }
 }
 
+// Threads of a block, of one of whole rows at most: it has as many warps as its row needs.
 template <int TPR> constexpr int kBlock = TPR > 32 ? TPR : 256;
+// Blocks a multiprocessor that the registers are held down for (0: as they come).
+template <int TPR, int E, bool SHIFT, bool BWD>
+constexpr int kResident = !SHIFT ? 0 : TPR <= 32 || TPR == 256 || TPR == 320 ? 2 : !BWD && TPR == 160 && E == 16 ? 3 : 0;
+template <int TPR> __device__ __forceinline__ int row_threads() { return TPR > 32 ? (int)blockDim.x : TPR; }
 
-// The pieces of a row that a thread has: piece k begins at column (k * TPR + lane) * VEC - shift.
+// The pieces of a row that a thread has: piece k begins at column (k * threads + lane) * VEC - shift.
+//
+// With SHIFT the first piece and the last one have places that are not the row's.  In x they get a value of the row's from
+// the same piece, which then counts n times too often: the sum takes n of them back, the sum of squares n of their
+// deviations' (which are no larger than what stays: nothing cancels).  In dy they are zero.
 template <typename T, int TPR, int K, bool SHIFT>
 struct RowPieces {
   static constexpr int VEC = kVec<T>, E = K * VEC;
-  int lane, width, shift;
+  int lane, threads, width, shift;
   int64_t rows;
+  float before, behind[K];   // places of the first piece, and of each other, that are not the row's
+  uint32_t own0[4], own1[4];  // the bits that are the row's: of piece 0, and of the last piece if that is another
 
-  __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * VEC - (SHIFT ? shift : 0); }
+  __device__ __forceinline__ RowPieces(int lane, int threads, int width, int shift, int64_t rows)
+      : lane(lane), threads(threads), width(width), shift(shift), rows(rows) {
+    before = SHIFT && lane == 0 && shift > 0 ? (float)(shift + max(0, VEC - shift - width)) : 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) behind[k] = SHIFT && any(k) && !first(k) ? (float)max(0, col(k) + VEC - width) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      own0[i] = SHIFT ? own(0, i) : 0;
+      own1[i] = 0;
+#pragma unroll
+      for (int k = 1; k < K; ++k)
+        if (SHIFT && any(k)) own1[i] = own(k, i);
+    }
+  }
+  __device__ __forceinline__ int col(int k) const { return (k * threads + lane) * VEC - (SHIFT ? shift : 0); }
   __device__ __forceinline__ bool any(int k) const { return col(k) < width; }
   __device__ __forceinline__ bool has(int k, int e) const {
     return SHIFT ? (unsigned)(col(k) + e) < (unsigned)width : any(k);
   }
-  // Whether some of the piece is not the row's: the first one's and the last one's lanes.
-  __device__ __forceinline__ bool edge(int k) const { return SHIFT && (col(k) < 0 || col(k) + VEC > width); }
+  // Whether some places of the piece are not the row's: before its first element, or behind its last one.
+  __device__ __forceinline__ bool first(int k) const { return SHIFT && k == 0 && col(0) < 0; }
+  __device__ __forceinline__ bool last(int k) const { return SHIFT && col(k) + VEC > width; }
+  __device__ __forceinline__ bool edge(int k) const { return any(k) && (first(k) || last(k)); }
+
   // Row `row` of `tensor`, zeros behind the last one.  (Nothing is read behind the tensor's end; before its beginning lies
   // nothing of a piece: the first row's shift is 0.)
   __device__ __forceinline__ void load(uint4* r, const void* tensor, int64_t ld, int64_t row) const {
-    const T* t = reinterpret_cast<const T*>(tensor);
-    const T *p = t + row * ld, *end = t + (rows - 1) * ld + width;
+    const T* p = reinterpret_cast<const T*>(tensor) + row * ld;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       r[k] = make_uint4(0, 0, 0, 0);
       if (row >= rows || !any(k)) continue;
-      if (SHIFT && p + col(k) + VEC > end) {
+      if (last(k) && row + VEC >= rows) {   // (VEC rows more are VEC elements at least)
         T t[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) t[e] = has(k, e) ? p[col(k) + e] : from_f32<T>(0.f);
@@ -122,40 +158,95 @@ struct RowPieces {
       }
     }
   }
-  // The values, 0 where they are not the row's.
+  // The bits of word i of piece k that are the row's.
+  __device__ __forceinline__ uint32_t own(int k, int i) const {
+    if constexpr (VEC == 4) return has(k, i) ? ~0u : 0u;
+    return (has(k, 2 * i) ? 0xffffu : 0u) | (has(k, 2 * i + 1) ? 0xffff0000u : 0u);
+  }
+  // The values; in the other places a value of the row's (FILL) or 0.
+  template <bool FILL>
   __device__ __forceinline__ void values(const uint4* r, float* f) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      unpack<T>(r[k], f + k * VEC);
+      uint4 v = r[k];
       if (edge(k)) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[k * VEC + e] = has(k, e) ? f[k * VEC + e] : 0.f;
+        uint32_t fill = 0;
+        if constexpr (FILL) {   // the piece's last value or its first one
+          fill = first(k) ? v.w : v.x;
+          if constexpr (VEC == 8) fill = __byte_perm(fill, 0, first(k) ? 0x3232 : 0x1010);
+          if (first(k) && last(k)) {
+            const int word = VEC == 4 ? shift : shift >> 1;
+            fill = word & 2 ? (word & 1 ? v.w : v.z) : (word & 1 ? v.y : v.x);
+            if constexpr (VEC == 8) fill = __byte_perm(fill, 0, shift & 1 ? 0x3232 : 0x1010);
+          }
+        }
+        const uint32_t* m = k == 0 ? own0 : own1;
+        v = make_uint4((v.x & m[0]) | (fill & ~m[0]), (v.y & m[1]) | (fill & ~m[1]), (v.z & m[2]) | (fill & ~m[2]), (v.w & m[3]) | (fill & ~m[3]));
       }
+      unpack<T>(v, f + k * VEC);
     }
   }
-  // f - mean, 0 where the value is not the row's.
+  // What the places that are not the row's have added to a sum of f, or of its squares.
+  __device__ __forceinline__ float sum(const float* f) const {
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) fadd2(s0, s1, s0, s1, f[e], f[e + 1]);
+    if constexpr (SHIFT) {
+      s0 = fmaf(-before, f[0], s0);
+#pragma unroll
+      for (int k = 0; k < K; ++k) s1 = fmaf(-behind[k], f[k * VEC + VEC - 1], s1);
+    }
+    return s0 + s1;
+  }
+  __device__ __forceinline__ float squares(const float* f) const {
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) ffma2(s0, s1, f[e], f[e + 1], f[e], f[e + 1], s0, s1);
+    if constexpr (SHIFT) {
+      s0 = fmaf(-before * f[0], f[0], s0);
+#pragma unroll
+      for (int k = 0; k < K; ++k) s1 = fmaf(-behind[k] * f[k * VEC + VEC - 1], f[k * VEC + VEC - 1], s1);
+    }
+    return s0 + s1;
+  }
+  // f - mean; pieces behind the row stay 0.
   __device__ __forceinline__ void center(float* f, float mean) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const float m = any(k) ? mean : 0.f;
 #pragma unroll
       for (int e = 0; e < VEC; e += 2) fadd2(f[k * VEC + e], f[k * VEC + e + 1], f[k * VEC + e], f[k * VEC + e + 1], -m, -m);
-      if (edge(k)) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[k * VEC + e] = has(k, e) ? f[k * VEC + e] : 0.f;
-      }
     }
   }
   __device__ __forceinline__ void store(T* p, const float* f) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!any(k)) continue;
-      if (edge(k)) {
+      T* to = p + col(k);
+      const uint4 v = pack<T>(f + k * VEC);
+      if (!edge(k)) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else if (first(k) && last(k)) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (has(k, e)) p[col(k) + e] = from_f32<T>(f[k * VEC + e]);
+          if (has(k, e)) to[e] = from_f32<T>(f[k * VEC + e]);
       } else {
-        *reinterpret_cast<uint4*>(p + col(k)) = pack<T>(f + k * VEC);
+        // in halves, quarters and eighths of the piece: from its place `shift` on, or as far as the row goes
+        const bool from = first(k);
+        const int n = from ? VEC - shift : width - col(k), h = VEC / 2, q = VEC / 4;
+        if (n & h) *reinterpret_cast<uint2*>(to + (from ? h : 0)) = from ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y);
+        const bool upper = ((n & h) != 0) != from;   // the half that the rest lies in
+        if (n & q) {
+          const uint32_t lo = upper ? v.z : v.x, hi = upper ? v.w : v.y;
+          *reinterpret_cast<uint32_t*>(to + (upper ? h : 0) + (from ? q : 0)) = from ? hi : lo;
+        }
+        if constexpr (VEC == 8) {
+          if (n & 1) {
+            const int at = from ? shift : n - 1, word = at >> 1;
+            const uint32_t w = word & 2 ? (word & 1 ? v.w : v.z) : (word & 1 ? v.y : v.x);
+            reinterpret_cast<unsigned short*>(to)[at] = (unsigned short)(at & 1 ? w >> 16 : w);
+          }
+        }
       }
     }
   }
@@ -180,13 +271,6 @@ __device__ __forceinline__ BlockRows block_rows(const LayerNormArgs& a, int vec,
 }
 
 template <int E>
-__device__ __forceinline__ float sum_of(const float* f) {
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) fadd2(s0, s1, s0, s1, f[e], f[e + 1]);
-  return s0 + s1;
-}
-template <int E>
 __device__ __forceinline__ float dot_of(const float* f, const float* g) {
   float s0 = 0.f, s1 = 0.f;
 #pragma unroll
@@ -195,15 +279,16 @@ __device__ __forceinline__ float dot_of(const float* f, const float* g) {
 }
 
 template <typename T, int TPR, int K, int R, bool SHIFT>
-__global__ void __launch_bounds__(kBlock<TPR>) layer_norm_fwd_kernel(LayerNormArgs a) {
+__global__ void __launch_bounds__(kBlock<TPR>, (kResident<TPR, K * kVec<T>, SHIFT, false>)) layer_norm_fwd_kernel(LayerNormArgs a) {
   constexpr int kGroups = kBlock<TPR> / TPR;
   using P = RowPieces<T, TPR, K, SHIFT>;
   constexpr int E = P::E;
   __shared__ float buf[2][R][32];
-  const int grp = threadIdx.x / TPR;
+  const int grp = TPR > 32 ? 0 : threadIdx.x / TPR;
   const BlockRows rows = block_rows<SHIFT>(a, kVec<T>, kGroups * R);
-  const P p{(int)(threadIdx.x % TPR), a.width, rows.shift, a.rows};
+  const P p((int)(threadIdx.x - grp * TPR), row_threads<TPR>(), a.width, rows.shift, a.rows);
   const float inv_width = 1.f / (float)a.width;
+  no_sums<TPR, R>(buf);
   after_previous();
   float w[E], b[E];
   p.affine(a.weight, a.affine_dtype, 1.f, w);
@@ -221,15 +306,15 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_fwd_kernel(LayerNormAr
     float f[R][E], mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      p.values(raw[r], f[r]);
-      mean[r] = sum_of<E>(f[r]);
+      p.template values<true>(raw[r], f[r]);
+      mean[r] = p.sum(f[r]);
     }
     if (base + rows.stride < a.rows) load(base + rows.stride);   // on their way meanwhile
     row_sums<TPR, R>(mean, buf[0]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       p.center(f[r], mean[r] * inv_width);
-      rstd[r] = dot_of<E>(f[r], f[r]);
+      rstd[r] = p.squares(f[r]);
     }
     row_sums<TPR, R>(rstd, buf[1]);
 #pragma unroll
@@ -247,15 +332,16 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_fwd_kernel(LayerNormAr
 }
 
 template <typename T, int TPR, int K, int R, bool SHIFT>
-__global__ void __launch_bounds__(kBlock<TPR>) layer_norm_bwd_kernel(LayerNormArgs a) {
+__global__ void __launch_bounds__(kBlock<TPR>, (kResident<TPR, K * kVec<T>, SHIFT, true>)) layer_norm_bwd_kernel(LayerNormArgs a) {
   constexpr int kGroups = kBlock<TPR> / TPR;
   using P = RowPieces<T, TPR, K, SHIFT>;
   constexpr int E = P::E, VEC = P::VEC;
   __shared__ float buf[2][2 * R][32];
-  const int grp = threadIdx.x / TPR;
+  const int grp = TPR > 32 ? 0 : threadIdx.x / TPR;
   const BlockRows rows = block_rows<SHIFT>(a, VEC, kGroups * R);
-  const P p{(int)(threadIdx.x % TPR), a.width, rows.shift, a.rows};
+  const P p((int)(threadIdx.x - grp * TPR), row_threads<TPR>(), a.width, rows.shift, a.rows);
   const float inv_width = 1.f / (float)a.width;
+  no_sums<TPR, 2 * R>(buf);
   after_previous();
   float w[E], dw[E], db[E];
   p.affine(a.weight, a.affine_dtype, 1.f, w);
@@ -275,9 +361,9 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_bwd_kernel(LayerNormAr
     float f[R][E], d[R][E], s[2 * R], t[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      p.values(raw_x[r], f[r]);
-      p.values(raw_dy[r], d[r]);     // (0 behind the last row)
-      s[2 * r] = sum_of<E>(f[r]);
+      p.template values<true>(raw_x[r], f[r]);
+      p.template values<false>(raw_dy[r], d[r]);     // (0 behind the last row)
+      s[2 * r] = p.sum(f[r]);
       s[2 * r + 1] = dot_of<E>(d[r], w);
     }
     if (base + rows.stride < a.rows) load(base + rows.stride);   // on their way meanwhile
@@ -292,7 +378,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_bwd_kernel(LayerNormAr
         fmul2(g0, g1, d[r][e], d[r][e + 1], w[e], w[e + 1]);
         ffma2(t0, t1, g0, g1, f[r][e], f[r][e + 1], t0, t1);
       }
-      t[2 * r] = dot_of<E>(f[r], f[r]);
+      t[2 * r] = p.squares(f[r]);
       t[2 * r + 1] = t0 + t1;
     }
     row_sums<TPR, 2 * R>(t, buf[1]);
@@ -463,19 +549,41 @@ cudaError_t sum_blocks(const LayerNormArgs& a, int blocks, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ dispatch
-// Threads a row and elements a thread, by the elements of its pieces.
+// Threads a row (of a whole block: at most) and elements a thread, by the elements of its pieces.
 struct RowShape {
   int tpr, e;
 };
+// Sixteen elements a thread where the registers allow it: fewer sums between threads.  The masks of SHIFT cost up to 25
+// registers, so its rows of fp32 (four pieces of sixteen elements) take eight up to 256, and its wide rows more threads of
+// eight, or one row at a time of two blocks a multiprocessor: a block alone waits at its sums with nothing beside it
+// (32,768 rows of 4095: bf16 forward 484 us with 512 threads for their 288, 203 with eight elements, 137 so).
+template <typename T, bool SHIFT, bool BWD>
 constexpr RowShape row_shape(int width) {
+  constexpr bool f32 = std::is_same<T, float>::value;
+  if (SHIFT && f32 && width <= 256)
+    return width <= 32 ? RowShape{4, 8} : width <= 64 ? RowShape{8, 8} : width <= 128 ? RowShape{16, 8} : RowShape{32, 8};
+  if (SHIFT && width > 2560 && width <= 5120) {
+    if (!f32 && !BWD) return {320, 16};
+    if (f32 || width > 4096) return {640, 8};
+  }
+  if (!SHIFT && f32 && BWD && width > 4096 && width <= 5120) return {640, 8};
   return width <= 64 ? RowShape{4, 16}
          : width <= 128 ? RowShape{8, 16}
          : width <= 256 ? RowShape{16, 16}
          : width <= 512 ? RowShape{32, 16}
-         : width <= 1024 ? RowShape{128, 8}
-         : width <= 2048 ? RowShape{128, 16}
+         : width <= 1280 ? RowShape{160, 8}
+         : width <= 2560 ? RowShape{160, 16}
          : width <= 4096 ? RowShape{256, 16}
                          : RowShape{512, 16};
+}
+// (all of its bounds are multiples of 32)
+template <typename T, bool SHIFT, bool BWD>
+constexpr bool shape_used(int tpr, int e) {
+  for (int w = 32; w <= kMaxRow; w += 32) {
+    const RowShape r = row_shape<T, SHIFT, BWD>(w);
+    if (r.tpr == tpr && r.e == e) return true;
+  }
+  return false;
 }
 // Classes of rows that begin at the same place of a 16-byte piece, and the elements of a row's pieces.
 int row_classes(int width, int vec) {
@@ -491,7 +599,10 @@ int pieces_width(int width, int vec) { return row_classes(width, vec) > 1 ? widt
 constexpr int most_blocks(int tpr) { return 148 * (tpr > 32 ? 3 : 8); }
 
 int64_t bwd_blocks(int64_t rows, int width, int vec) {
-  const int tpr = row_shape(pieces_width(width, vec)).tpr, classes = row_classes(width, vec);
+  const int classes = row_classes(width, vec), w = pieces_width(width, vec);
+  const RowShape r = vec == 4 ? (classes > 1 ? row_shape<float, true, true>(w) : row_shape<float, false, true>(w))
+                              : (classes > 1 ? row_shape<__half, true, true>(w) : row_shape<__half, false, true>(w));
+  const int tpr = r.tpr;
   const int64_t per = tpr > 32 ? 1 : 256 / tpr, b = (rows + per - 1) / per;
   const int64_t most = b < most_blocks(tpr) ? b : most_blocks(tpr);
   return (most + classes - 1) / classes * classes;
@@ -499,44 +610,60 @@ int64_t bwd_blocks(int64_t rows, int width, int vec) {
 
 template <auto Kernel>
 int blocks_per_sm(int threads) {
-  static std::atomic<int> known{0};
-  int b = known.load(std::memory_order_relaxed);
+  static std::atomic<int> known[32];   // by the block's warps
+  int b = known[threads / 32].load(std::memory_order_relaxed);
   if (b == 0) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, Kernel, threads, 0) != cudaSuccess || b < 1) b = 1;
-    known.store(b, std::memory_order_relaxed);
+    known[threads / 32].store(b, std::memory_order_relaxed);
   }
   return b;
 }
 
 template <typename T, int TPR, int E, bool SHIFT, bool BWD>
 cudaError_t launch_row(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
-  // rows that a group of threads works on at a time; in the backward two where it is a block of 128, which waits
+  // rows that a group of threads works on at a time; in the backward two where it is a block of up to 160, which waits
   // for all of its threads twice a turn (more threads leave no registers for it)
-  constexpr int kThreads = kBlock<TPR>, R = BWD && TPR != 128 ? 1 : 2, K = E / kVec<T>;
+  constexpr int R = (BWD && TPR != 160) || TPR == 320 ? 1 : 2, K = E / kVec<T>;
+  const int pieces = (pieces_width(a.width, kVec<T>) + kVec<T> - 1) / kVec<T>;
+  const int threads = TPR > 32 ? (pieces + 32 * K - 1) / (32 * K) * 32 : kBlock<TPR>;
   constexpr auto kern = [] {
     if constexpr (BWD) return &layer_norm_bwd_kernel<T, TPR, K, R, SHIFT>;
     else return &layer_norm_fwd_kernel<T, TPR, K, R, SHIFT>;
   }();
-  const int64_t per = (int64_t)(kThreads / TPR) * R, need = (a.rows + per - 1) / per;
-  int64_t most = (int64_t)sm_count() * blocks_per_sm<kern>(kThreads);
+  const int64_t per = (TPR > 32 ? 1 : threads / TPR) * R, need = (a.rows + per - 1) / per;
+  int64_t most = (int64_t)sm_count() * blocks_per_sm<kern>(threads);
   if (BWD && most > most_blocks(TPR)) most = most_blocks(TPR);
-  if (need < most) most = need;
-  *blocks = (int)(SHIFT ? (most + a.classes - 1) / a.classes * a.classes : most);
-  return launch_early(kern, dim3((unsigned)*blocks), kThreads, 0, s, a);
+  // whole classes of blocks, and no more than run at a time: a few that came after the others would double the time
+  const int64_t classes = SHIFT ? a.classes : 1, all = (need + classes - 1) / classes * classes;
+  most = most < classes ? classes : most / classes * classes;
+  *blocks = (int)(all < most ? all : most);
+  return launch_early(kern, dim3((unsigned)*blocks), threads, 0, s, a);
 }
 
 template <typename T, bool SHIFT, bool BWD>
 cudaError_t launch_width(const LayerNormArgs& a, cudaStream_t s, int* blocks) {
-  const RowShape r = row_shape(pieces_width(a.width, kVec<T>));
-  switch (r.tpr) {
-    case 4: return launch_row<T, 4, 16, SHIFT, BWD>(a, s, blocks);
-    case 8: return launch_row<T, 8, 16, SHIFT, BWD>(a, s, blocks);
-    case 16: return launch_row<T, 16, 16, SHIFT, BWD>(a, s, blocks);
-    case 32: return launch_row<T, 32, 16, SHIFT, BWD>(a, s, blocks);
-    case 128: return r.e == 8 ? launch_row<T, 128, 8, SHIFT, BWD>(a, s, blocks) : launch_row<T, 128, 16, SHIFT, BWD>(a, s, blocks);
-    case 256: return launch_row<T, 256, 16, SHIFT, BWD>(a, s, blocks);
-    default: return launch_row<T, 512, 16, SHIFT, BWD>(a, s, blocks);
-  }
+  const RowShape r = row_shape<T, SHIFT, BWD>(pieces_width(a.width, kVec<T>));
+  cudaError_t error = cudaErrorInvalidValue;
+  auto with = [&](auto tpr, auto e) {
+    constexpr int TPR = decltype(tpr)::value, E = decltype(e)::value;
+    if constexpr (shape_used<T, SHIFT, BWD>(TPR, E))
+      if (r.tpr == TPR && r.e == E) error = launch_row<T, TPR, E, SHIFT, BWD>(a, s, blocks);
+  };
+  using std::integral_constant;
+  auto both = [&](auto tpr) {
+    with(tpr, integral_constant<int, 8>{});
+    with(tpr, integral_constant<int, 16>{});
+  };
+  both(integral_constant<int, 4>{});
+  both(integral_constant<int, 8>{});
+  both(integral_constant<int, 16>{});
+  both(integral_constant<int, 32>{});
+  both(integral_constant<int, 160>{});
+  both(integral_constant<int, 256>{});
+  both(integral_constant<int, 320>{});
+  both(integral_constant<int, 512>{});
+  both(integral_constant<int, 640>{});
+  return error;
 }
 
 template <typename T, bool BWD>
