@@ -65,7 +65,7 @@ struct Params {
   int y_tma;
   float* partials;
   int64_t partial_stride;
-  int splits, add;
+  int splits, split_tiles, add;
   unsigned int* status;
 };
 
@@ -95,8 +95,10 @@ __device__ __forceinline__ TileAt tile_at(const Params& p, int t, int rank) {
   r.job = 0;
   r.split = 0;
   if constexpr (MODE == kWeight) {
-    r.split = t % p.splits;
-    t /= p.splits;
+    // (one split after the other: its rows of the operands stay in L2 for all of its tiles.  The splits of a tile side by
+    // side read all rows anew in every round, 235 MB of 8192 rows, width 1024, hidden 4096)
+    r.split = t / p.split_tiles;
+    t -= r.split * p.split_tiles;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       if (r.job == j && t >= p.m_tiles[j] * p.n_tiles[j]) {
@@ -696,6 +698,7 @@ cudaError_t launch_group(const GemmArgs& g, cudaStream_t stream) {
   p.partials = g.partials;
   p.partial_stride = g.partial_stride;
   p.splits = g.splits;
+  p.split_tiles = MODE == kWeight ? (int)(tiles / g.splits) : 0;
   p.add = g.add;
   p.status = g.status;
   constexpr auto kern = ff_gemm_kernel<T, PARTS, OUT, MODE, NT, B_MN, CG>;
@@ -753,18 +756,20 @@ cudaError_t gemm(const GemmArgs& g, cudaStream_t s) {
   return g.bf16 ? dispatch<__nv_bfloat16, 1, __nv_bfloat16>(g, s) : dispatch<__half, 1, __half>(g, s);
 }
 
-// The number of splits whose rounds of tiles over the SMs cost least (a split's last reads and writes
-// are counted as 1/32 of a round); at least 256 rows a split.
+// The number of splits whose rounds of tiles over the SMs cost least, at least 256 rows a split.  A round costs its rows,
+// and as much as kTail rows more for writing its sums and reading them again: 74 pairs' 256 x 256 are 19 MB, both ways
+// 6 us, in which they do about 1000 rows (fp32, six products a row: 170).
 int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms) {
   const bool wide = wide_tiles(f32, {n[0], n[1], n[2]});
   const int cg = weight_pairs(f32, {m[0], m[1], m[2]}) ? 2 : 1;
   int64_t tiles = 0;
   for (int j = 0; j < 3; ++j) tiles += tiles_of(m[j], 128 * cg) * tiles_of(n[j], wide ? 256 : 128);
   sms /= cg;
+  const float kTail = f32 ? 170.f : 1000.f;
   int best = 1;
   float cost = 1e30f;
   for (int s = 1; s <= 32 && (s == 1 || rows / s >= 256); ++s) {
-    const float c = (float)tiles_of(tiles * s, sms) * (1.f / s + 1.f / 32);
+    const float c = (float)tiles_of(tiles * s, sms) * ((float)rows / s + kTail);
     if (c < cost) {
       cost = c;
       best = s;
