@@ -36,6 +36,31 @@ def test_shapes(shape, shared, dtype):
     check(x, None, 0.15, 5, 0, shared)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shared", [-3, -2])
+@pytest.mark.parametrize("shape", [(2, 9, 1), (40, 37, 5), (3, 11, 9), (70, 17, 9), (17, 65, 10), (6, 200, 23), (1, 301, 12), (301, 3, 31),
+                                   (33, 41, 127), (5, 90, 130), (3, 3, 2047)])
+def test_rows_inside_pieces(shape, shared, dtype):
+    """Rows of every alignment, tiny ones, several turns and steps of a thread; the other rows of a piece keep their own."""
+    x, r = normal(*shape, seed=1, dtype=dtype), normal(*shape, seed=2, dtype=dtype)
+    check(x, r, 0.3, -7, 1, shared)
+    check(x, None, 0.6, 5, 0, shared)
+
+
+def test_nothing_behind_a_map_is_written():
+    """Results of rows that end inside a piece, in a larger buffer of the caller's."""
+    from trifast_b200 import _lib
+    n, c = 5, 27
+    x = normal(n, n, c, seed=1, dtype=torch.bfloat16)
+    y = torch.full((x.numel() + 16,), 3.0, device="cuda", dtype=x.dtype)
+    keep = oracle.keep_mask(x.shape, 0.5, 3, 0, -2).cuda()
+    d = _lib.Dropout(outer=n, mid=n, inner=c, dtype=_lib.DTYPE_CODE[x.dtype], p=0.5, seed=3, offset=0)
+    rc = _lib.load().trifast_dropout_add(d, None, x.data_ptr(), None, y.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "dropout")
+    assert torch.equal(y[:x.numel()].view_as(x), torch.where(keep, 2 * x, torch.zeros_like(x)))
+    assert (y[x.numel():] == 3).all()
+
+
 @pytest.mark.parametrize("shared", [None, 0, 1, 2, 3])
 def test_batched_maps_and_strides(shared):
     x = normal(2, 6, 5, 40, seed=1, dtype=torch.bfloat16)

@@ -13,6 +13,7 @@
 // round and scheduler for two chains of two products).
 
 #include "block_kernels.h"
+#include "pieces.cuh"
 #include "tc_common.cuh"
 
 namespace trifast {
@@ -109,6 +110,20 @@ __device__ __forceinline__ uint4 apply(uint4 x, const uint4& res, const uint4& m
 
 __device__ __forceinline__ uint64_t key_of(const DropoutArgs& a) { return a.seed + (a.seed_ptr ? (uint64_t)*a.seed_ptr : 0); }
 
+// Eight words from any entry on (of which those before 0 mean nothing).
+__device__ __forceinline__ void words8_at(int64_t entry, uint64_t offset, uint64_t key, uint32_t* w) {
+  uint32_t all[12];
+#pragma unroll
+  for (int b = 0; b < 3; ++b) {
+    const Words q = philox((uint64_t)((entry >> 2) + b), offset, key);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) all[4 * b + e] = q.w[e];
+  }
+  const int skip = (int)(entry & 3);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = skip & 2 ? (skip & 1 ? all[e + 3] : all[e + 2]) : (skip & 1 ? all[e + 1] : all[e]);
+}
+
 // Shared masks whose inner extent is a multiple of eight: a thread has eight columns and `walk` steps of mid, `mids`
 // apart.  Columns run fastest over the threads, then the first `mids` steps of mid, then outer.
 template <typename T, bool RES>
@@ -199,9 +214,69 @@ __global__ void __launch_bounds__(256) dropout_own_kernel(DropoutArgs a) {
   }
 }
 
-// Shared masks of other inner extents: a thread has one column.
+// Shared masks of other inner extents: the rows (o, m) begin inside 16-byte pieces, at the same place for every
+// `classes`-th m.  A thread has eight places that begin with a piece and the steps m0, m0 + mids, ... of mid, `mids` a
+// multiple of the classes: it reads whole pieces and writes what the row has of them.  (1024 x 1024 x 127 bf16 with one mask
+// for all columns and a residual: 148 us; one column a thread 279; 128 columns 132.)
 template <typename T, bool RES>
-__global__ void __launch_bounds__(256) dropout_column_kernel(DropoutArgs a, int64_t mids, int walk) {
+__global__ void __launch_bounds__(256) dropout_shift_kernel(DropoutArgs a, int64_t cols, int64_t mids) {
+  constexpr int U = 2, N = kPieces<T>, V = 16 / sizeof(T);   // steps in flight, pieces and elements of one
+  after_previous();
+  const uint64_t key = key_of(a);
+  const int64_t total = a.outer * mids * cols, step = mids * a.inner;
+  const T *xs = reinterpret_cast<const T*>(a.x), *rs = reinterpret_cast<const T*>(a.residual);
+  const int64_t end = a.outer * a.mid * a.inner;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t p = i % cols, om = i / cols, m0 = om % mids, o = om / mids;
+    if (m0 >= a.mid) continue;
+    const int64_t row = (o * a.mid + m0) * a.inner;
+    const int shift = (int)(row % V);
+    const int64_t col = p * 8 - shift;
+    if (col >= a.inner) continue;
+    uint32_t w[8];
+    words8_at(o * a.inner + col, a.offset, key, w);
+    const Eight<T> mask = keep_mask<T>(w, a.threshold);
+    int lo[N], hi[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      lo[k] = (int)max((int64_t)0, -col - k * V);
+      hi[k] = (int)min((int64_t)V, a.inner - col - k * V);
+    }
+    auto load = [&](const T* t, int64_t e) {   // nothing behind the tensor's end
+      if (e + V <= end) return *reinterpret_cast<const uint4*>(t + e);
+      T v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = e + j < end ? t[e + j] : from_f32<T>(0.f);
+      uint4 u;
+      memcpy(&u, v, 16);
+      return u;
+    };
+    int64_t e = row + col;
+    for (int64_t m = m0; m < a.mid; m += U * mids, e += U * step) {
+      uint4 vx[U][N], vr[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (m + u * mids < a.mid)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (hi[k] > 0) {
+              vx[u][k] = load(xs, e + u * step + k * V);
+              if (RES) vr[u][k] = load(rs, e + u * step + k * V);
+            }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (m + u * mids < a.mid)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (hi[k] > 0)
+              store_part(reinterpret_cast<T*>(a.y) + e + u * step + k * V, apply<T, RES>(vx[u][k], vr[u][k], mask.v[k], a.scale), lo[k], hi[k]);
+    }
+  }
+}
+
+// Shared masks of few places, of which the pieces would be edges for the most part: a thread has one column.
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256) dropout_column_kernel(DropoutArgs a, int64_t mids) {
   after_previous();
   const uint64_t key = key_of(a);
   const int64_t total = a.outer * mids * a.inner;
@@ -227,6 +302,9 @@ unsigned blocks_for(int64_t threads, int64_t most) {
   return (unsigned)(b < most ? b : most);
 }
 
+// (1000 x 1000 maps with one mask for all columns, bf16, a column a thread and in pieces: 9 places 20 and 24 us, 33 84 and 52)
+constexpr int kShiftInner = 16;
+
 template <typename T, bool RES>
 cudaError_t launch_type(DropoutArgs a, cudaStream_t s) {
   const int64_t sms = sm_count();
@@ -236,16 +314,19 @@ cudaError_t launch_type(DropoutArgs a, cudaStream_t s) {
     const int64_t threads = a.inner / 16 > a.inner % 8 ? a.inner / 16 : a.inner % 8;
     return launch_early(dropout_own_kernel<T, RES>, dim3(blocks_for(threads < 1 ? 1 : threads, sms * 8)), 256, 0, s, a);
   }
-  const bool whole = a.inner % 8 == 0;
-  const int64_t cols = whole ? a.inner / 8 : a.inner, lanes = a.outer * cols;
+  const bool whole = a.inner % 8 == 0, few = a.inner < kShiftInner;
+  const int vec = 16 / (int)sizeof(T), classes = row_classes(a.inner, vec);
+  const int64_t cols = whole ? a.inner / 8 : few ? a.inner : (a.inner + vec - 1 + 7) / 8, lanes = a.outer * cols;
   // Steps of mid that a thread walks with one mask: as many as leave eight blocks of 256 threads a multiprocessor.
   int64_t walk = lanes * a.mid / (sms * 8 * 256);
   walk = walk < 1 ? 1 : walk > 64 ? 64 : walk;
   if (walk > a.mid) walk = a.mid;
-  const int64_t mids = (a.mid + walk - 1) / walk;
+  int64_t mids = (a.mid + walk - 1) / walk;
+  if (!whole && !few) mids = (mids + classes - 1) / classes * classes;
   const unsigned blocks = blocks_for(lanes * mids, 1 << 30);
   if (whole) return launch_early(dropout_shared_kernel<T, RES>, dim3(blocks), 256, 0, s, a, cols, mids, (int)walk);
-  return launch_early(dropout_column_kernel<T, RES>, dim3(blocks), 256, 0, s, a, mids, (int)walk);
+  if (few) return launch_early(dropout_column_kernel<T, RES>, dim3(blocks), 256, 0, s, a, mids);
+  return launch_early(dropout_shift_kernel<T, RES>, dim3(blocks), 256, 0, s, a, cols, mids);
 }
 
 }  // namespace

@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "block_kernels.h"
+#include "pieces.cuh"
 #include "tc_common.cuh"
 
 namespace trifast {
@@ -224,30 +225,8 @@ struct RowPieces {
       if (!any(k)) continue;
       T* to = p + col(k);
       const uint4 v = pack<T>(f + k * VEC);
-      if (!edge(k)) {
-        *reinterpret_cast<uint4*>(to) = v;
-      } else if (first(k) && last(k)) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (has(k, e)) to[e] = from_f32<T>(f[k * VEC + e]);
-      } else {
-        // in halves, quarters and eighths of the piece: from its place `shift` on, or as far as the row goes
-        const bool from = first(k);
-        const int n = from ? VEC - shift : width - col(k), h = VEC / 2, q = VEC / 4;
-        if (n & h) *reinterpret_cast<uint2*>(to + (from ? h : 0)) = from ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y);
-        const bool upper = ((n & h) != 0) != from;   // the half that the rest lies in
-        if (n & q) {
-          const uint32_t lo = upper ? v.z : v.x, hi = upper ? v.w : v.y;
-          *reinterpret_cast<uint32_t*>(to + (upper ? h : 0) + (from ? q : 0)) = from ? hi : lo;
-        }
-        if constexpr (VEC == 8) {
-          if (n & 1) {
-            const int at = from ? shift : n - 1, word = at >> 1;
-            const uint32_t w = word & 2 ? (word & 1 ? v.w : v.z) : (word & 1 ? v.y : v.x);
-            reinterpret_cast<unsigned short*>(to)[at] = (unsigned short)(at & 1 ? w >> 16 : w);
-          }
-        }
-      }
+      if (!edge(k)) *reinterpret_cast<uint4*>(to) = v;
+      else store_part(to, v, first(k) ? shift : 0, min(VEC, width - col(k)));
     }
   }
   __device__ __forceinline__ void affine(const void* a, int dtype, float otherwise, float* w) const {
@@ -585,15 +564,7 @@ constexpr bool shape_used(int tpr, int e) {
   }
   return false;
 }
-// Classes of rows that begin at the same place of a 16-byte piece, and the elements of a row's pieces.
-int row_classes(int width, int vec) {
-  int c = vec;
-  while (c > 1 && width % 2 == 0) {
-    width /= 2;
-    c /= 2;
-  }
-  return c;
-}
+// The elements of a row's pieces.
 int pieces_width(int width, int vec) { return row_classes(width, vec) > 1 ? width + vec - 1 : width; }
 // Blocks of the backward at most: eight a multiprocessor (three of whole rows, whose partial sums are wide).
 constexpr int most_blocks(int tpr) { return 148 * (tpr > 32 ? 3 : 8); }
