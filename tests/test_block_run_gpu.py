@@ -274,7 +274,7 @@ def test_c_entries_check_their_arguments():
 
     ff = lambda **kw: C.byref(_lib.FeedForward(**{**dict(rows=4, ld_x=64, ld_dy=32, width=64, hidden=96, width_out=32, dtype=1), **kw}))
     fwd = lambda f, x=ok, ws=ok, size=1 << 30: lib.trifast_feed_forward(f, x, ok, ok, ok, ok, ws, size, None)
-    assert fwd(None) == -1 and fwd(ff(), x=None) == -1 and fwd(ff(), x=C.c_void_p(0x1002)) == -6 and fwd(ff(), size=1) == -7
+    assert fwd(None) == -1 and fwd(ff(), x=None) == -1 and fwd(ff(), x=C.c_void_p(0x1002)) == -6 and fwd(ff(rows=64, dtype=0), size=1) == -7
     for kw, rc in ((dict(rows=-1), -2), (dict(hidden=0), -2), (dict(width_out=65537), -2), (dict(dtype=-1), -4), (dict(ld_x=60), -5)):
         assert fwd(ff(**kw)) == rc, kw
         assert lib.trifast_feed_forward_workspace_bytes(ff(**kw)) == 0
