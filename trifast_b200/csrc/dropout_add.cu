@@ -214,10 +214,13 @@ __global__ void __launch_bounds__(256) dropout_own_kernel(DropoutArgs a) {
   }
 }
 
+// (1000 x 1000 maps with one mask for all columns, bf16, a column a thread and in pieces: 9 places 20 and 23 us, 33 84 and 49)
+constexpr int kShiftInner = 16;
+
 // Shared masks of other inner extents: the rows (o, m) begin inside 16-byte pieces, at the same place for every
 // `classes`-th m.  A thread has eight places that begin with a piece and the steps m0, m0 + mids, ... of mid, `mids` a
 // multiple of the classes: it reads whole pieces and writes what the row has of them.  (1024 x 1024 x 127 bf16 with one mask
-// for all columns and a residual: 148 us; one column a thread 279; 128 columns 132.)
+// for all columns and a residual: 137 us; one column a thread 279; 128 columns 132.)
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_shift_kernel(DropoutArgs a, int64_t cols, int64_t mids) {
   constexpr int U = 2, N = kPieces<T>, V = 16 / sizeof(T);   // steps in flight, pieces and elements of one
@@ -268,8 +271,14 @@ __global__ void __launch_bounds__(256) dropout_shift_kernel(DropoutArgs a, int64
         if (m + u * mids < a.mid)
 #pragma unroll
           for (int k = 0; k < N; ++k)
-            if (hi[k] > 0)
-              store_part(reinterpret_cast<T*>(a.y) + e + u * step + k * V, apply<T, RES>(vx[u][k], vr[u][k], mask.v[k], a.scale), lo[k], hi[k]);
+            if (hi[k] > 0) {   // (a row of kShiftInner places ends in another piece than it begins in)
+              T* to = reinterpret_cast<T*>(a.y) + e + u * step + k * V;
+              const uint4 v = apply<T, RES>(vx[u][k], vr[u][k], mask.v[k], a.scale);
+              if (lo[k] == 0 && hi[k] == V)
+                *reinterpret_cast<uint4*>(to) = v;
+              else
+                store_part(to, v, lo[k] > 0, lo[k] > 0 ? V - lo[k] : hi[k]);
+            }
     }
   }
 }
@@ -301,9 +310,6 @@ unsigned blocks_for(int64_t threads, int64_t most) {
   const int64_t b = (threads + 255) / 256;
   return (unsigned)(b < most ? b : most);
 }
-
-// (1000 x 1000 maps with one mask for all columns, bf16, a column a thread and in pieces: 9 places 20 and 24 us, 33 84 and 52)
-constexpr int kShiftInner = 16;
 
 template <typename T, bool RES>
 cudaError_t launch_type(DropoutArgs a, cudaStream_t s) {

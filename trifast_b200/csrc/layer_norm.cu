@@ -225,8 +225,15 @@ struct RowPieces {
       if (!any(k)) continue;
       T* to = p + col(k);
       const uint4 v = pack<T>(f + k * VEC);
-      if (!edge(k)) *reinterpret_cast<uint4*>(to) = v;
-      else store_part(to, v, first(k) ? shift : 0, min(VEC, width - col(k)));
+      if (!edge(k)) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else if (first(k) && last(k)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (has(k, e)) to[e] = from_f32<T>(f[k * VEC + e]);
+      } else {
+        store_part(to, v, first(k), first(k) ? VEC - shift : width - col(k));
+      }
     }
   }
   __device__ __forceinline__ void affine(const void* a, int dtype, float otherwise, float* w) const {
@@ -566,8 +573,8 @@ constexpr bool shape_used(int tpr, int e) {
 }
 // The elements of a row's pieces.
 int pieces_width(int width, int vec) { return row_classes(width, vec) > 1 ? width + vec - 1 : width; }
-// Blocks of the backward at most: eight a multiprocessor (three of whole rows, whose partial sums are wide).
-constexpr int most_blocks(int tpr) { return 148 * (tpr > 32 ? 3 : 8); }
+// Blocks of the backward at most: eight a multiprocessor (three of wide rows, whose partial sums are wide too).
+constexpr int most_blocks(int tpr) { return 148 * (tpr > 160 ? 3 : 8); }
 
 int64_t bwd_blocks(int64_t rows, int width, int vec) {
   const int classes = row_classes(width, vec), w = pieces_width(width, vec);
