@@ -12,88 +12,108 @@ namespace {
 
 // Matrices with rows of 16-byte pitch, and fp32 as three bf16 planes.  A value is cut, not rounded, to its upper 8
 // significant bits, and what is left again: the three parts hold its 24 bits exactly and have one sign.  A thread makes
-// eight columns of a row: it reads the aligned 16-byte pieces that they lie in and shifts them into place (element by
-// element, the loads of 6280 x 913 bf16 and its weights took 12.6 us).  Columns behind the last are zero.
+// eight columns of a row, kUnits times, all read before the first is written: it reads the aligned 16-byte pieces that they lie
+// in and shifts them into place (element by element, the loads of 6280 x 913 bf16 and its weights took 12.6 us).  Columns
+// behind the last are zero.  The pieces of all rows run over the lanes (262,144 x 65 bf16 17.4 us; 55 with 16 lanes for the nine pieces of a row, one at a time).
+template <typename T> constexpr int kUnits = sizeof(T) == 2 ? 4 : 2;
 struct StageJobs {
   StageJob job[kStageJobs];
-  int64_t end[kStageJobs];    // warps up to and with each
-  int lanes[kStageJobs];      // lanes of a row: 4 to 32
+  int64_t end[kStageJobs];    // warps' turns up to and with each
   int count;
 };
 template <typename T>
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ StageJobs jobs) {
   constexpr int kElem = sizeof(T), W = 2 * kElem, V = W / 4 + 1;   // words of eight columns; pieces that they can lie in
+  constexpr int U = kUnits<T>;
   after_previous();
+  const int lane = threadIdx.x & 31;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < jobs.end[jobs.count - 1]; i += (int64_t)gridDim.x * 8) {
     int j = 0;
     while (i >= jobs.end[j]) ++j;
     const StageJob& job = jobs.job[j];
-    const int lanes = jobs.lanes[j], lane = threadIdx.x & 31;
-    const int64_t r = (i - (j ? jobs.end[j - 1] : 0)) * (32 / lanes) + lane / lanes;
-    if (r >= job.rows) continue;
     const int cols = (int)job.dst.cols, pieces = (int)(job.dst.pitch / 8);
-    const T* src = reinterpret_cast<const T*>(job.src) + r * job.ld;
-    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);   // the same for all pieces of the row
     const char* end = reinterpret_cast<const char*>(reinterpret_cast<const T*>(job.src) + (job.rows - 1) * job.ld + cols);
-    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(job.dst.p) + r * job.dst.pitch);
-    for (int p = lane % lanes; p < pieces; p += lanes) {
-      const int there = cols - 8 * p < 8 ? cols - 8 * p : 8;   // columns of this piece (at least one)
-      uint32_t w[4 * V];
-      const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(src) - off) + p * (V - 1);
+    const int64_t first = (i - (j ? jobs.end[j - 1] : 0)) * (32 * U), row0 = first / pieces;
+    const uint32_t rest = (uint32_t)(first - row0 * pieces);
+    uint32_t w[U][4 * V];
+    int64_t row[U];
+    int piece[U];
+    uint32_t off[U];   // bytes before its eight columns
+    auto load = [&](int64_t row, int piece, uint32_t (&x)[4 * V], uint32_t& off) {
+      const T* src = reinterpret_cast<const T*>(job.src) + row * job.ld;
+      off = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);
+      const int there = min(cols - 8 * piece, 8);   // columns of this piece (at least one)
+      const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(src) - off) + piece * (V - 1);
       const int used = ((int)off + there * kElem + 15) / 16;   // pieces that hold something of the row
       if (reinterpret_cast<const char*>(from + used) <= end) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (v < used) u = from[v];
-          w[4 * v] = u.x;
-          w[4 * v + 1] = u.y;
-          w[4 * v + 2] = u.z;
-          w[4 * v + 3] = u.w;
-        }
-#pragma unroll
-        for (int k = 0; k < 4 * V; ++k) {
-          const uint32_t far = k + 2 < 4 * V ? w[k + 2] : 0;
-          w[k] = off & 8 ? far : w[k];
-        }
-#pragma unroll
-        for (int k = 0; k < 4 * V; ++k) {
-          const uint32_t next = k + 1 < 4 * V ? w[k + 1] : 0;
-          w[k] = off & 4 ? next : w[k];
-        }
-        if (kElem == 2)
-#pragma unroll
-          for (int k = 0; k < W; ++k) w[k] = off & 2 ? __funnelshift_r(w[k], w[k + 1], 16) : w[k];
+        for (int v = 0; v < V; ++v)
+          if (v < used) {
+            const uint4 q = from[v];
+            x[4 * v] = q.x;
+            x[4 * v + 1] = q.y;
+            x[4 * v + 2] = q.z;
+            x[4 * v + 3] = q.w;
+          }
       } else {
         // nothing is read behind the matrix's end
-#pragma unroll
-        for (int k = 0; k < W; ++k) w[k] = 0;
         T t[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = e < there ? src[8 * p + e] : from_f32<T>(0.f);
-        memcpy(w, t, sizeof(t));
+        for (int e = 0; e < 8; ++e) t[e] = e < there ? src[8 * piece + e] : from_f32<T>(0.f);
+        memcpy(x, t, sizeof(t));
+        off = 0;
       }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t t = rest + u * 32 + lane, rr = t / (uint32_t)pieces;
+      piece[u] = (int)(t - rr * pieces);
+      row[u] = row0 + rr;
+#pragma unroll
+      for (int k = 0; k < 4 * V; ++k) w[u][k] = 0;
+      off[u] = 0;
+      if (row[u] < job.rows) load(row[u], piece[u], w[u], off[u]);
+    }
+    auto put = [&](int64_t row, int piece, uint32_t (&x)[4 * V], uint32_t off) {
+      const int there = min(cols - 8 * piece, 8);
+#pragma unroll
+      for (int k = 0; k < 4 * V; ++k) {
+        const uint32_t far = k + 2 < 4 * V ? x[k + 2] : 0;
+        x[k] = off & 8 ? far : x[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4 * V; ++k) {
+        const uint32_t next = k + 1 < 4 * V ? x[k + 1] : 0;
+        x[k] = off & 4 ? next : x[k];
+      }
+      if (kElem == 2)
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[k] = off & 2 ? __funnelshift_r(x[k], x[k + 1], 16) : x[k];
+      uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(job.dst.p) + row * job.dst.pitch) + piece;
       if constexpr (kElem == 2) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = 2 * k + 1 < there ? w[k] : 2 * k < there ? w[k] & 0xffffu : 0u;
-        out[p] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 0; k < 4; ++k) x[k] = 2 * k + 1 < there ? x[k] : 2 * k < there ? x[k] & 0xffffu : 0u;
+        *out = make_uint4(x[0], x[1], x[2], x[3]);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = k < there ? w[k] : 0u;
+        for (int k = 0; k < 8; ++k) x[k] = k < there ? x[k] : 0u;
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-          uint32_t u[4];
+          uint32_t b[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            u[k] = __byte_perm(w[2 * k], w[2 * k + 1], 0x7632);
+            b[k] = __byte_perm(x[2 * k], x[2 * k + 1], 0x7632);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              w[2 * k + h] = __float_as_uint(__uint_as_float(w[2 * k + h]) - __uint_as_float(w[2 * k + h] & 0xffff0000u));
+              x[2 * k + h] = __float_as_uint(__uint_as_float(x[2 * k + h]) - __uint_as_float(x[2 * k + h] & 0xffff0000u));
           }
-          out[q * (job.dst.plane / 8) + p] = make_uint4(u[0], u[1], u[2], u[3]);
+          out[q * (job.dst.plane / 8)] = make_uint4(b[0], b[1], b[2], b[3]);
         }
       }
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (row[u] < job.rows) put(row[u], piece[u], w[u], off[u]);
   }
 }
 
@@ -154,15 +174,12 @@ dim3 grid_for(int64_t threads) {
 
 cudaError_t stage(const StageJob* jobs, int count, int dtype, cudaStream_t s) {
   StageJobs a = {};
+  const int64_t per = 32 * (dtype == TRIFAST_F32 ? kUnits<float> : kUnits<__half>);
   for (int j = 0; j < count; ++j) {
-    a.job[a.count] = jobs[j];
-    int lanes = 4;
-    while (lanes < 32 && lanes < jobs[j].dst.pitch / 8) lanes *= 2;
-    a.lanes[a.count] = lanes;
-    const int per = 32 / lanes;
-    a.end[a.count] = (a.count ? a.end[a.count - 1] : 0) + (jobs[j].rows + per - 1) / per;
-    ++a.count;
+    a.job[j] = jobs[j];
+    a.end[j] = (j ? a.end[j - 1] : 0) + (jobs[j].rows * (jobs[j].dst.pitch / 8) + per - 1) / per;
   }
+  a.count = count;
   if (count == 0) return cudaSuccess;
   const dim3 g = grid_for(a.end[count - 1] * 32);
   return dtype == TRIFAST_F32 ? launch_early(stage_kernel<float>, g, 256, 0, s, a) : launch_early(stage_kernel<__half>, g, 256, 0, s, a);
