@@ -97,6 +97,30 @@ def test_few_rows(rows, c, h, o, dtype):
         assert_bounded(gated_feed_forward(v, *w), want[0], bound[0], "y")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 3, 8])
+@pytest.mark.parametrize("c,h,o", [(289, 909, 301), (520, 1024, 1300), (601, 2048, 40), (1500, 24, 1200), (1111, 601, 7)])
+def test_few_rows_of_wide_blocks(rows, c, h, o, dtype):
+    """Two kernels: a warp or a block to a result, pieces or elements."""
+    from trifast_b200 import gated_feed_forward
+    dy, x, *w = draw(rows, c, h, o, dtype)
+    want, bound = bounds(dy, x, *w)
+    y = gated_feed_forward(x, *w)
+    assert_bounded(y, want[0], bound[0], "y")
+    assert torch.equal(y, gated_feed_forward(x, *w))
+
+
+@pytest.mark.parametrize("rows,c,dtype", [(45001, 136, torch.bfloat16), (45001, 131, torch.float16), (15003, 24, torch.float32)])
+def test_several_chunks_of_hidden_values(rows, c, dtype):
+    """Three chunks of rows in the workspace, whose weight gradients are added up, the same bits each time."""
+    from trifast_b200 import gated_feed_forward
+    dy, x, *w = draw(rows, c, 2048, c, dtype)
+    check(dy, x, *w)
+    leaves = [t.clone().requires_grad_() for t in (x, *w)]
+    run = lambda: torch.autograd.grad(gated_feed_forward(*leaves), leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(run(), run()))
+
+
 @pytest.mark.parametrize("dtype", DTYPES[:2])
 @pytest.mark.parametrize("rows,c,h,o", [
     (9472, 128, 512, 128), (9601, 128, 64, 128), (18945, 128, 130, 40), (20011, 40, 200, 128), (40003, 128, 64, 128),

@@ -1,7 +1,7 @@
 // The feed-forward block's forward pass for a few rows (a token or so at a time): both products on the CUDA cores, a
-// warp to a hidden unit and then to a result, which read every weight once.  Hidden values are fp32.
+// warp to a hidden unit and then a warp or a block to a result, which read every weight once.  Hidden values are fp32.
 //
-// What bounds it: the launches, and the latency of one read of the weights.  Small blocks (kClusterBytes of weights) are
+// What bounds it: the launches, and the latency of one read of the weights.  Small blocks (a megabyte of weights) are
 // one kernel, a cluster of eight CTAs whose warps write their hidden values into the shared memory of all eight; larger
 // ones two kernels over all multiprocessors.  (Width 128, hidden 512, one row: 11.0 us a call on the tensor-core
 // kernels, whose tiles are 128 rows, 9.5 as two kernels.)
@@ -47,6 +47,23 @@ __device__ __forceinline__ void warp_sum(float* v) {
     for (int r = 0; r < R; ++r) v[r] += __shfl_xor_sync(0xffffffffu, v[r], m);
 }
 
+// The sums of a block's eight warps, in all of them.
+template <int R>
+__device__ __forceinline__ void block_sum(float* v) {
+  __shared__ float sum[kWarps][R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane == r) sum[warp][r] = v[r];
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    v[r] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v[r] += sum[w][r];
+  }
+}
+
 // silu(x wg^T) * (x wu^T) of one hidden unit: in lane r that of row r
 template <typename T, int R, int N>
 __device__ __forceinline__ float unit_value(const T* __restrict__ x, int64_t ld, int rows, const T* __restrict__ wg, const T* __restrict__ wu,
@@ -77,12 +94,13 @@ __device__ __forceinline__ float unit_value(const T* __restrict__ x, int64_t ld,
   return h;
 }
 
-// One result: in lane r that of row r (h: rows `pitch` apart)
-template <typename T, int R, int N>
+// One result: in lane r that of row r (h: rows `pitch` apart).  BLOCK: by the eight warps of a block together.
+template <typename T, int R, int N, bool BLOCK>
 __device__ __forceinline__ float result_value(const float* h, int rows, const T* __restrict__ wd, int hidden, int pitch, int lane) {
+  constexpr int kLanes = BLOCK ? 32 * kWarps : 32;
   float s[R] = {};
 #pragma unroll 2
-  for (int c = lane * N; c < hidden; c += 32 * N) {
+  for (int c = (BLOCK ? (int)threadIdx.x : lane) * N; c < hidden; c += kLanes * N) {
     float w[N];
     read<T, N>(wd + c, w);
 #pragma unroll
@@ -94,6 +112,7 @@ __device__ __forceinline__ float result_value(const float* h, int rows, const T*
     }
   }
   warp_sum<R>(s);
+  if constexpr (BLOCK) block_sum<R>(s);
   float y = 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -111,13 +130,13 @@ __global__ void __launch_bounds__(32 * kWarps) few_hidden_kernel(FewArgs p) {
   if (lane < p.rows) p.h[lane * p.pitch + unit] = h;
 }
 
-template <typename T, int R, int N>
+template <typename T, int R, int N, bool BLOCK>
 __global__ void __launch_bounds__(32 * kWarps) few_result_kernel(FewArgs p) {
   after_previous();
-  const int o = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int o = BLOCK ? blockIdx.x : blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (o >= p.width_out) return;
-  const float y = result_value<T, R, N>(p.h, p.rows, (const T*)p.wd + (int64_t)o * p.hidden, p.hidden, p.pitch, lane);
-  if (lane < p.rows) ((T*)p.y)[(int64_t)lane * p.width_out + o] = from_f32<T>(y);
+  const float y = result_value<T, R, N, BLOCK>(p.h, p.rows, (const T*)p.wd + (int64_t)o * p.hidden, p.hidden, p.pitch, lane);
+  if ((BLOCK ? (int)threadIdx.x : lane) < p.rows) ((T*)p.y)[(int64_t)lane * p.width_out + o] = from_f32<T>(y);
 }
 
 // Both, by a cluster.  N, M: neighbours read at a time along the width and along the hidden units.
@@ -140,7 +159,7 @@ __global__ void __launch_bounds__(kClusterThreads) few_cluster_kernel(FewArgs p)
   }
   cluster_sync();
   for (int o = warp; o < p.width_out; o += kClusterWarps) {
-    const float y = result_value<T, R, M>(few_h, p.rows, (const T*)p.wd + (int64_t)o * p.hidden, p.hidden, p.pitch, lane);
+    const float y = result_value<T, R, M, false>(few_h, p.rows, (const T*)p.wd + (int64_t)o * p.hidden, p.hidden, p.pitch, lane);
     if (lane < p.rows) ((T*)p.y)[(int64_t)lane * p.width_out + o] = from_f32<T>(y);
   }
 }
@@ -154,10 +173,16 @@ cudaError_t launch(const FewArgs& a, cudaStream_t s) {
                                                                                                         : few_cluster_kernel<T, R, 1, 1>;
     return launch_clusters(kern, dim3(kClusterCtas), kClusterThreads, (size_t)a.rows * a.pitch * sizeof(float), s, kClusterCtas, a);
   }
-  const int units = (a.hidden + kWarps - 1) / kWarps, results = (a.width_out + kWarps - 1) / kWarps;
-  const cudaError_t e = launch_early(in ? few_hidden_kernel<T, R, N> : few_hidden_kernel<T, R, 1>, dim3(units), 32 * kWarps, 0, s, a);
+  const cudaError_t e =
+      launch_early(in ? few_hidden_kernel<T, R, N> : few_hidden_kernel<T, R, 1>, dim3((a.hidden + kWarps - 1) / kWarps), 32 * kWarps, 0, s, a);
   if (e != cudaSuccess) return e;
-  return launch_early(out ? few_result_kernel<T, R, N> : few_result_kernel<T, R, 1>, dim3(results), 32 * kWarps, 0, s, a);
+  // A block to a result where a warp to each would be too few for the device and read for long (bf16, 8 rows, width 1024,
+  // hidden 4096: 14 us, a warp 21; 6 rows, 801 and 3001: 13 and 86.  The hidden units are more and their rows shorter: a block
+  // to each took 11.7 us for 6.3, 5 rows, 289 and 909.)
+  const bool block = a.width_out <= 148 * kWarps && a.hidden > 64 * (out ? N : 1);
+  const auto result = block ? (out ? few_result_kernel<T, R, N, true> : few_result_kernel<T, R, 1, true>)
+                            : (out ? few_result_kernel<T, R, N, false> : few_result_kernel<T, R, 1, false>);
+  return launch_early(result, dim3(block ? a.width_out : (a.width_out + kWarps - 1) / kWarps), 32 * kWarps, 0, s, a);
 }
 
 template <typename T>
