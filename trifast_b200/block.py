@@ -82,7 +82,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     and so are their gradients in the backward, which computes the hidden values again instead of keeping
     them: nothing but the arguments is saved, and the workspace of a call does not grow with the number of
     rows.  fp32 products are as exact as fp32 sums, but a row with an infinite value in x or a weight gives
-    NaN there.  Differentiable, once, in all four.
+    NaN there.  The forward pass of up to eight rows runs on the CUDA cores with fp32 hidden values: its last
+    bits may differ from those of the same rows in a larger batch.  Differentiable, once, in all four.
     """
     return _gated_feed_forward(x, w_gate, w_up, w_down)
 
