@@ -14,7 +14,8 @@ namespace {
 // significant bits, and what is left again: the three parts hold its 24 bits exactly and have one sign.  A thread makes
 // eight columns of a row, kUnits times, all read before the first is written: it reads the aligned 16-byte pieces that they lie
 // in and shifts them into place (element by element, the loads of 6280 x 913 bf16 and its weights took 12.6 us).  Columns
-// behind the last are zero.  The pieces of all rows run over the lanes (262,144 x 65 bf16 17.4 us; 55 with 16 lanes for the nine pieces of a row, one at a time).
+// behind the last are zero.  The pieces of all rows run over the lanes (262,144 x 65 bf16: 17.4 us; 55 with 16 lanes for
+// the nine pieces of a row, one at a time).
 template <typename T> constexpr int kUnits = sizeof(T) == 2 ? 4 : 2;
 struct StageJobs {
   StageJob job[kStageJobs];
