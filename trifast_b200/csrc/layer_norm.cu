@@ -371,7 +371,9 @@ __global__ void __launch_bounds__(kBlock<TPR>, (kResident<TPR, K * kVec<T>, SHIF
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = base + (r * kGroups + grp) * rows.step;
-      const float rstd = rsqrtf(fmaf(t[2 * r], inv_width, a.eps)), m1 = s[2 * r + 1] * inv_width, m2 = t[2 * r + 1] * rstd * inv_width;
+      // (0 behind the last row: its zeros have no variance, and without an eps the inverse of that would reach dw)
+      const float rstd = row < a.rows ? rsqrtf(fmaf(t[2 * r], inv_width, a.eps)) : 0.f;
+      const float m1 = s[2 * r + 1] * inv_width, m2 = t[2 * r + 1] * rstd * inv_width;
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
         float &x0 = f[r][e], &x1 = f[r][e + 1], &d0 = d[r][e], &d1 = d[r][e + 1];
