@@ -65,7 +65,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension.
 
-    x: (..., width), fp32, bf16 or fp16; weight and bias: (width,), both of x's type or both fp32, or None
+    x: (..., width), fp32, bf16 or fp16, with width at most 2**20; weight and bias: (width,), both of x's type or both fp32, or None
     (no affine part; a bias needs a weight).  Arithmetic is in fp32 and the result, of x's shape and type,
     is rounded once.  Differentiable, once, in x, weight and bias.  Rows may be strided; a tensor whose
     leading dimensions cannot be walked with one stride is copied.

@@ -93,6 +93,8 @@ optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(
 trifast_norm check_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must be (..., width); got ", x.sizes());
   const int64_t width = x.size(-1);
+  // (before it is held in 32 bits)
+  TORCH_CHECK_VALUE(width <= 1 << 20, "width must be at most 1048576; got ", width);
   for (const auto& [name, t] : {std::pair{"weight", &weight}, std::pair{"bias", &bias}}) {
     if (!t->defined()) continue;
     TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == width, name, " must be [", width, "]; got ", t->sizes());
