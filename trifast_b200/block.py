@@ -3,7 +3,8 @@ block ("transition"), and dropout with the residual sum.
 
 Native like the attention (``csrc/torch_block_ops.cpp``): argument checks, allocation and autograd run
 without Python, all compute in the CUDA library behind the C ABI, on the caller's stream; nothing
-synchronises, and calls can be captured in a CUDA graph.  A pre-norm block of a pair map ``z`` of shape
+synchronises, and calls can be captured in a CUDA graph.  Gradients are those of reverse mode; an input with
+a forward-mode tangent is refused (NotImplementedError).  A pre-norm block of a pair map ``z`` of shape
 (*batch, n, n, width)::
 
     z = dropout_add(attention(layer_norm(z, w0, b0)), z, p, seed, shared_dim=-3)

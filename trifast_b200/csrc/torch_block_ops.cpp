@@ -19,6 +19,7 @@ using std::optional;
 using trifast_torch::check_rc;
 using trifast_torch::dtype_code;
 using trifast_torch::raise_if_device_gave_up;
+using trifast_torch::refuse_tangents;
 
 // ------------------------------------------------------------------ arguments
 void check_like(const char* name, const Tensor& t, const Tensor& x) {
@@ -198,6 +199,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm_autograd(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
   const Tensor w = value(weight), b = value(bias);
+  refuse_tangents("layer_norm", {&x, &w, &b});
   if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   return call_norm(x, weight, bias, eps);
@@ -222,6 +224,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_grads_autograd(const Tensor& dy, c
                                                              double eps, bool wx, bool ww, bool wb) {
   static auto op = find_op<NormGradsSig>("trifast_b200::layer_norm_grads");
   const Tensor w = value(weight);
+  refuse_tangents("layer_norm_grads", {&dy, &x, &w});
   if (wants_grad({&dy, &x, &w})) {
     const variable_list r = NormOnce::apply(dy, x, weight, eps, wx, ww, wb);
     return {r[0], r[1], r[2]};
@@ -333,6 +336,7 @@ class FeedForward : public torch::autograd::Function<FeedForward> {
 };
 
 Tensor feed_forward_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd) {
+  refuse_tangents("gated_feed_forward", {&x, &wg, &wu, &wd});
   if (wants_grad({&x, &wg, &wu, &wd})) return FeedForward::apply(x, wg, wu, wd);
   at::AutoDispatchBelowADInplaceOrView below;
   return call_ff(x, wg, wu, wd);
@@ -355,6 +359,7 @@ class FfOnce : public torch::autograd::Function<FfOnce> {
 std::tuple<Tensor, Tensor, Tensor, Tensor> feed_forward_grads_autograd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
                                                                        const Tensor& wd, bool wx, bool ww) {
   static auto op = find_op<FfGradsSig>("trifast_b200::gated_feed_forward_grads");
+  refuse_tangents("gated_feed_forward_grads", {&dy, &x, &wg, &wu, &wd});
   if (wants_grad({&dy, &x, &wg, &wu, &wd})) {
     const variable_list r = FfOnce::apply(dy, x, wg, wu, wd, wx, ww);
     return {r[0], r[1], r[2], r[3]};
@@ -434,6 +439,7 @@ class DropoutAdd : public torch::autograd::Function<DropoutAdd> {
 Tensor dropout_add_autograd(const Tensor& x, const optional<Tensor>& residual, double p, int64_t seed, int64_t offset,
                             const optional<Tensor>& seed_tensor, optional<int64_t> shared_dim) {
   const Tensor r = value(residual);
+  refuse_tangents("dropout_add", {&x, &r});
   if (wants_grad({&x, &r})) return DropoutAdd::apply(x, residual, p, seed, offset, seed_tensor, shared_dim);
   at::AutoDispatchBelowADInplaceOrView below;
   return call_dropout(x, residual, p, seed, offset, seed_tensor, shared_dim);

@@ -64,6 +64,12 @@ void raise_if_device_gave_up(c10::DeviceIndex dev, cudaStream_t stream) {
                       : "(the status could not be cleared here, as during a graph capture)");
 }
 
+void refuse_tangents(const char* op, std::initializer_list<const at::Tensor*> inputs) {
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "trifast_b200::", op,
+                                " has no forward-mode derivative");
+}
+
 }  // namespace trifast_torch
 
 namespace {
