@@ -57,3 +57,28 @@ def test_forward_over_reverse_is_refused():
     y = layer_norm(x)
     with fwd.dual_level(), pytest.raises(NotImplementedError, match="no forward-mode derivative"):
         torch.autograd.grad(y, x, fwd.make_dual(torch.empty_like(y), torch.empty_like(y)))
+
+
+# ------------------------------------------------------------------ the attention
+Q, B, M = meta(1, 2, 5, 5, 16), meta(1, 2, 5, 5), meta(1, 5, 5, dtype=torch.bool)
+SAVED = (Q, Q, Q, Q, B, Q, meta(1, 2, 5, 5))
+ATTENTION = {
+    "triangle_attention": (lambda *a: trifast_b200.triangle_attention(*a, M), (Q, Q, Q, B)),
+    "triangle_attention_ending_node": (lambda *a: trifast_b200.triangle_attention_ending_node(*a, M), (Q, Q, Q, B)),
+    "triangle_attention_grads": (lambda *a: ops.triangle_attention_grads(*a, M), SAVED),
+    "triangle_attention_backward": (lambda *a: ops.triangle_attention_backward(*a, M), SAVED),
+}
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("name,place", [(n, i) for n, (_, args) in ATTENTION.items() for i in range(len(args))])
+def test_attention_refuses_tangents(name, place, requires_grad):
+    call, args = ATTENTION[name]
+    refused(call, args, place, requires_grad)
+
+
+@pytest.mark.parametrize("name", ATTENTION)
+def test_attention_refuses_jvp(name):
+    call, args = ATTENTION[name]
+    with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+        torch.func.jvp(call, args, tuple(torch.empty_like(a) for a in args))

@@ -78,6 +78,7 @@ using at::Tensor;
 using trifast_torch::check_rc;
 using trifast_torch::dtype_code;
 using trifast_torch::raise_if_device_gave_up;
+using trifast_torch::refuse_tangents;
 
 // ------------------------------------------------------------------ arguments
 struct Problem {
@@ -318,6 +319,7 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 
 std::tuple<Tensor, Tensor> forward_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const Tensor& b, const Tensor& mask) {
+  refuse_tangents("triangle_attention", {&q, &k, &v, &b});
   if (!wants_grad({&q, &k, &v, &b})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_forward(q, k, v, b, mask);
@@ -347,6 +349,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> grads_autograd(const Tensor& d_o, con
                                                           const Tensor& k, const Tensor& v,
                                                           const Tensor& b, const Tensor& o,
                                                           const Tensor& lse, const Tensor& mask) {
+  refuse_tangents("triangle_attention_grads", {&d_o, &q, &k, &v, &b, &o, &lse});
   if (wants_grad({&d_o, &q, &k, &v, &b, &o, &lse})) {
     const variable_list r = Once::apply(d_o, q, k, v, b, o, lse, mask);
     return {r[0], r[1], r[2], r[3]};
@@ -359,6 +362,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> grads_autograd(const Tensor& d_o, con
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> backward_autograd(
     const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& b,
     const Tensor& o, const Tensor& lse, const Tensor& mask) {
+  refuse_tangents("triangle_attention_backward", {&d_o, &q, &k, &v, &b, &o, &lse});
   if (wants_grad({&d_o, &q, &k, &v, &b, &o, &lse})) {
     const variable_list r = Once::apply(d_o, q, k, v, b, o, lse, mask);
     return {r[0], r[1], r[2], r[3], at::zeros_like(mask)};

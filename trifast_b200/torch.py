@@ -147,7 +147,8 @@ def triangle_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: tor
     ``*batch`` is any number of leading dimensions, including none (the reference
     takes exactly one, src/trifast/torch.py:29 notes the rest as to do); they are
     folded into one batch dimension for the kernels.  Returns o with the shape and
-    dtype of q.  Differentiable in q, k, v and b.
+    dtype of q.  Differentiable in q, k, v and b, in reverse mode
+    (an input with a forward-mode tangent is refused).
     """
     if q.dim() == 5:
         o, _ = _triangle_attention(q, k, v, b, mask)
