@@ -113,6 +113,12 @@ __device__ __forceinline__ void repeat_status(unsigned int* status) {
   const unsigned int bits = *reinterpret_cast<volatile unsigned int*>(status);
   if (bits != 0u) mirror_status(status, bits);
 }
+// Whether an earlier kernel on this device has given up, for a kernel that is then to do nothing.  All threads of the block
+// call this, before any of them returns, and get the answer that one of them has read: threads that read the word for
+// themselves may see it change in between, and those that left would be missing at the others' barriers.
+__device__ __forceinline__ bool block_gave_up(unsigned int* status) {
+  return __syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<volatile unsigned int*>(status) != 0u) != 0;
+}
 __device__ __forceinline__ void set_status(unsigned int* status, unsigned int bits) {
   mirror_status(status, atomicOr(status, bits) | bits);
 }

@@ -21,9 +21,9 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
-// Whether an earlier kernel on this device has given up: the kernels then write nothing, and tell the host word again.
+// block_gave_up(), and the host word is told again.
 __device__ __forceinline__ bool device_gave_up(unsigned int* status) {
-  const bool up = *reinterpret_cast<volatile unsigned int*>(status) != 0u;
+  const bool up = block_gave_up(status);
   if (up && blockIdx.x == 0 && threadIdx.x == 0) repeat_status(status);
   return up;
 }
