@@ -18,15 +18,19 @@ def source(name):
         return f.read()
 
 
-@pytest.mark.parametrize("name", ["ff_gemm.cu", "ff_fused.cu"])
+@pytest.mark.parametrize("name", ["ff_gemm.cu", "ff_fused.cu", "tc_bwd_d128.cu", "tc_bwd_db.cu", "tc_bwd_dkv.cu", "tc_bwd_dq.cu", "tc_bwd_fused.cu",
+                                  "tc_fwd.cu", "tc_fwd_d128.cu"])
 def test_status_is_read_once_a_block(name):
     """A thread that reads the word for itself may see it set where others of its block have not: it would leave them
     waiting at a barrier that counts on it."""
     direct = r"volatile unsigned int\*>\((p\.)?status"
     helper = source("common.cuh").split("bool block_gave_up(")[1].split("}")[0]
-    assert "__syncthreads_or(threadIdx.x == 0 &&" in helper and re.search(direct, helper)
-    assert "block_gave_up(status)" in source("ff_device.cuh") and not re.search(direct, source("ff_device.cuh"))
+    assert "return __syncthreads_or(" in helper and re.search(direct, helper)
+    assert "= block_gave_up(status, threadIdx.x == 0);" in source("ff_device.cuh") and not re.search(direct, source("ff_device.cuh"))
     text = source(name)
+    if name == "tc_bwd_db.cu":     # (with clusters one thread hands what it has read to the others in shared memory)
+        text, ours = re.subn(r"if \(kCluster\) \*skip = \*reinterpret_cast<volatile unsigned int\*>\(status\) != 0u;", "", text)
+        assert ours == 1
     assert not re.search(direct, text)
     assert len(re.findall(r"__global__", text)) == len(re.findall(r"(device|block)_gave_up\((p\.)?status\)", text))
 
@@ -57,3 +61,23 @@ def test_every_product_after_a_kernel_that_gave_up(rows, width, hidden, dtype):
     with pytest.raises(RuntimeError, match="gave up"):
         gated_feed_forward(x, *w)
     assert torch.equal(gated_feed_forward(x, *w), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d", [(64, 16), (128, 32), (200, 64), (384, 32), (128, 128)])
+def test_attention_after_a_kernel_that_gave_up(n, d):
+    """The backward's kernels end together too: the call after it raises, and the one after that is right."""
+    from trifast_b200 import _lib, triangle_attention
+    lib = _lib.load()
+    q, k, v, do = (normal(1, 2, n, n, d, seed=s, dtype=torch.bfloat16) for s in range(4))
+    b, m = normal(1, 2, n, n, seed=5, dtype=torch.bfloat16), torch.zeros(1, n, n, dtype=torch.bool, device="cuda")
+    o, lse = torch.ops.trifast_b200.triangle_attention(q, k, v, b, m)
+    grads = lambda: torch.ops.trifast_b200.triangle_attention_grads(do, q, k, v, b, o, lse, m)
+    want = [t.clone() for t in grads()]
+    torch.cuda.synchronize()
+    _lib.check(lib.trifast_debug_wait_probe(1000, C.c_void_p(torch.cuda.current_stream().cuda_stream)), "trifast_debug_wait_probe")
+    grads()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="gave up"):
+        triangle_attention(q, k, v, b, m)
+    assert all(torch.equal(a, b) for a, b in zip(grads(), want))

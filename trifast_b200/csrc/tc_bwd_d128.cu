@@ -156,7 +156,7 @@ tc_bwd_d128_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_cons
   }
   after_previous();
 
-  if (*reinterpret_cast<volatile unsigned int*>(status) != 0u) return;
+  if (block_gave_up(status)) return;
 
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   if (tid == 0) {

@@ -141,7 +141,7 @@ tc_db_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   after_previous();
 
   // (a cluster's CTAs must all reach its barriers: they skip the rows instead)
-  if (!kCluster && *reinterpret_cast<volatile unsigned int*>(status) != 0u) return;
+  if (!kCluster && block_gave_up(status)) return;
   volatile int* skip = reinterpret_cast<volatile int*>(gbase + 264);
 
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;

@@ -120,7 +120,7 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   };
   auto slot_row = [&](const Item& it, int r) -> int { return min(it.i0 + r, dm.n_rows - 1); };
 
-  if (*reinterpret_cast<volatile unsigned int*>(status) != 0u) return;
+  if (block_gave_up(status)) return;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 

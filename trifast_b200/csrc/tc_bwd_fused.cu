@@ -192,7 +192,7 @@ tc_dqkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   }
   after_previous();
 
-  if (*reinterpret_cast<volatile unsigned int*>(status) != 0u) return;
+  if (block_gave_up(status)) return;
 
   // (what every lane of a warp shares goes through uniform(), so that the compiler keeps it, and the
   // descriptors made of it, in uniform registers, where the MMAs want them)

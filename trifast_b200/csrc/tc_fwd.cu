@@ -169,7 +169,7 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
 
   // A wait that gave up in an earlier CTA or launch leaves the status word set:
   // stop doing work until the host has read and cleared it.
-  if (*reinterpret_cast<volatile unsigned int*>(status) != 0u) {
+  if (block_gave_up(status)) {
     if (threadIdx.x == 0) repeat_status(status);   // (no prepare kernel runs before small problems)
     return;
   }

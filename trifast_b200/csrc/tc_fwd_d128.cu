@@ -120,7 +120,7 @@ tc_fwd_d128_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   }
   after_previous();
 
-  if (*reinterpret_cast<volatile unsigned int*>(status) != 0u) return;
+  if (block_gave_up(status)) return;
 
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
