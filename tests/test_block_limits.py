@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests.test_block_run_gpu import on_cuda_kernel
+from trifast_b200 import _lib
 
 WIDTHS = [(1 << 20) + 1, 1 << 31, (1 << 32) + 8, (1 << 33) + 64]
 
@@ -24,3 +25,14 @@ def test_feed_forward_refuses_wide_rows(width):
     x, g, d = torch.empty(0, width), torch.empty(1, 1).expand(1, width), torch.zeros(4, 1)
     with pytest.raises(ValueError, match="at most 65536"):
         on_cuda_kernel("gated_feed_forward", x, g, g, d)
+
+
+def test_weight_sums_have_a_share_of_the_workspace_for_each_run():
+    """Without a device: rows of a chunk beyond 128 tiles have partial sums of their own."""
+    lib = _lib.load()
+    size = lambda rows, w, h, dt: lib.trifast_feed_forward_backward_workspace_bytes(C.byref(_lib.FeedForward(rows, w, w, w, h, w, dt)))
+    for width, hidden in ((136, 8), (200, 16)):
+        stride = 4 * (2 * hidden * width + width * hidden)
+        for rows in (128 * 128 * 40, 128 * 128 * 100):
+            values = 3 * 2 * hidden * (-(-rows // 128) * 128)      # h, da, db of the chunk
+            assert size(rows, width, hidden, 2) - values >= stride * (rows // (128 * 128))

@@ -1,11 +1,12 @@
 """The gated feed-forward block where its arithmetic ends: gates whose exponential overflows, hidden values beyond
-the largest fp16 number, and gradients near the smallest."""
+the largest fp16 number, gradients near the smallest, and sums over millions of rows."""
 
 import pytest
 import torch
 
 from tests.block_helpers import DTYPES, STEP, TINY, U, assert_bounded, normal
 from tests.test_feed_forward_gpu import bounds, draw, run
+from oracle import block_oracle as oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +73,32 @@ def test_small_gradients(std, c, dtype):
     want, bound = bounds(dy, x, *w)
     for name, g, e, b in zip(("y", "dx", "dw_gate", "dw_up", "dw_down"), run(dy, x, *w), want, bound):
         assert_bounded(g, e, b, name)
+
+
+@pytest.mark.parametrize("c,hidden", [(136, 8), (128, 64), (64, 40)])
+def test_sums_of_millions_of_rows_do_not_drift(c, hidden):
+    """Weight gradients over 5.5 million rows, every term positive.  The accumulators of TMEM round towards zero, so that a
+    long sum drifts.  A run of sums there is 128 row tiles, 1024 additions of 16 products; if each loses two steps of 2^-23,
+    of an accumulator that is half its last value on average, the mean over the entries is off by 1024 2^-23 = 1.22e-4, a
+    quarter of fp16's rounding.  What the entries' own roundings (u = 2^-11, a uniform error of u / sqrt 3) leave in that mean is
+    below 6 u / sqrt(3 count)."""
+    from trifast_b200 import gated_feed_forward
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    rows = 5_500_000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rand = lambda *s: torch.rand(*s, generator=g, device="cuda")
+    x, dy = (0.5 + rand(rows, c)).half(), (0.004 + 0.002 * rand(rows, c)).half()
+    wg, wu = ((rand(hidden, c) / 64).half() for _ in range(2))
+    wd = (rand(c, hidden) / 32).half()
+    leaves = [t.requires_grad_() for t in (wg, wu, wd)]
+    got = torch.autograd.grad(gated_feed_forward(x, *leaves), leaves, dy)
+    want = [torch.zeros(t.shape, dtype=torch.float64, device="cuda") for t in leaves]
+    for r in range(0, rows, 500_000):
+        for s, v in zip(want, oracle.feed_forward_grads(dy[r:r + 500_000], x[r:r + 500_000], *(t.detach() for t in leaves))[1:]):
+            s += v
+    off = torch.cat([((p.double() - q) / q).flatten() for p, q in zip(got, want)])
+    assert max(float(q.max()) for q in want) * (1 + 2.0 ** -10) < 65504 and min(float(q.min()) for q in want) > 1
+    mean = float(off.mean())
+    print(f"mean relative error of {off.numel()} sums: {mean:.3g}")
+    assert abs(mean) <= 1024 * 2.0 ** -23 + 6 * U[torch.float16] / (3 * off.numel()) ** 0.5

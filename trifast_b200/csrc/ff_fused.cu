@@ -544,10 +544,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) ff_dx_kernel(const __grid_cons
 }
 
 // ------------------------------------------------------------------ dWg, dWu, dWd
-// A CTA has a chunk of hidden units and a share of the row tiles, in runs of at most kRun, after each of which its sums
-// go to memory (the accumulators of TMEM round towards zero: 8 MMAs a tile, so a run's drift is about 5e-5 of
-// the sum).  TMEM: S [0, 128) and [128, 256), dH [256, 320), [dWg; dWu] [320, 320 + CP), dWd [448, 512).
-constexpr int kRun = 512;
+// A CTA has a chunk of hidden units and a share of the row tiles, in runs of at most kRunTiles, after each of which its sums
+// go to memory.  TMEM: S [0, 128) and [128, 256), dH [256, 320), [dWg; dWu] [320, 320 + CP), dWd [448, 512).
 template <int CP>
 struct Weights {   // (warps of this kernel: 0-7 elementwise, 8 TMA, 9 and 10 MMA issuers: S and dH; the gradients)
   static constexpr int kX = CP / 64 * kTile, kStage = 2 * kX;
@@ -661,8 +659,8 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
     for (int t = 0; t < count && ok; ++t) {
       // (the rows are there: S and dH have read them)
       ok = wait(STG_READY, t & 1);
-      const int in_run = t % kRun;
-      if (ok && in_run == 0 && t > 0) ok = wait(ACC_FREE, (t / kRun - 1) & 1);
+      const int in_run = t % kRunTiles;
+      if (ok && in_run == 0 && t > 0) ok = wait(ACC_FREE, (t / kRunTiles - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -678,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
           umma_ss(tmem + 448, dy + k * (2048 >> 4), h + k * (2048 >> 4), make_idesc(128, 64, kBf16, true, true), (in_run > 0 || k > 0) ? 1u : 0u);
         umma_commit(sm.bar(DY_EMPTY + (t & 1)));
         umma_commit(sm.bar(STG_FREE));
-        if (in_run == kRun - 1 || t == count - 1) umma_commit(sm.bar(ACC_DONE));
+        if (in_run == kRunTiles - 1 || t == count - 1) umma_commit(sm.bar(ACC_DONE));
       }
       __syncwarp();
     }
@@ -736,11 +734,11 @@ __global__ void __launch_bounds__(kThreads, 1) ff_dw_kernel(const __grid_constan
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.bar(STG_READY));
-      if (t % kRun == kRun - 1 || t == count - 1) {
-        ok = wait(ACC_DONE, (t / kRun) & 1);
+      if (t % kRunTiles == kRunTiles - 1 || t == count - 1) {
+        ok = wait(ACC_DONE, (t / kRunTiles) & 1);
         if (!ok) break;
         tc_fence_after();
-        flush(t >= kRun || p.add);
+        flush(t >= kRunTiles || p.add);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(sm.bar(ACC_FREE));

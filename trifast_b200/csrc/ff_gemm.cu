@@ -758,7 +758,8 @@ cudaError_t gemm(const GemmArgs& g, cudaStream_t s) {
 
 // The number of splits whose rounds of tiles over the SMs cost least, at least 256 rows a split.  A round costs its rows,
 // and as much as kTail rows more for writing its sums and reading them again: 74 pairs' 256 x 256 are 19 MB, both ways
-// 6 us, in which they do about 1000 rows (fp32, six products a row: 170).
+// 6 us, in which they do about 1000 rows (fp32, six products a row: 170).  16-bit types: no split is longer than a run of
+// sums (fp32 adds up in registers).
 int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, int sms) {
   const bool wide = wide_tiles(f32, {n[0], n[1], n[2]});
   const int cg = weight_pairs(f32, {m[0], m[1], m[2]}) ? 2 : 1;
@@ -766,9 +767,10 @@ int weight_splits(const int64_t* m, const int64_t* n, int64_t rows, bool f32, in
   for (int j = 0; j < 3; ++j) tiles += tiles_of(m[j], 128 * cg) * tiles_of(n[j], wide ? 256 : 128);
   sms /= cg;
   const float kTail = f32 ? 170.f : 1000.f;
-  int best = 1;
+  const int64_t run = (int64_t)kRunTiles * 128, least = f32 ? 1 : (rows + run - 1) / run, most = least > 16 ? 2 * least : 32;
+  int best = (int)least;
   float cost = 1e30f;
-  for (int s = 1; s <= 32 && (s == 1 || rows / s >= 256); ++s) {
+  for (int s = best; s <= most && (s == least || rows / s >= 256); ++s) {
     const float c = (float)tiles_of(tiles * s, sms) * ((float)rows / s + kTail);
     if (c < cost) {
       cost = c;
