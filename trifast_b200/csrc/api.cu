@@ -2,6 +2,7 @@
 // carving and dispatch to the kernel launchers.  Entry points are declared and
 // documented in include/trifast_b200.h.
 
+#include <cuda.h>
 #include <float.h>
 #include <math.h>
 #include <stddef.h>
@@ -28,6 +29,20 @@ unsigned int* g_host_word[kMaxDevices];   // pinned mirrors of the status words 
 cudaError_t g_host_word_error[kMaxDevices];
 std::once_flag g_host_word_once[kMaxDevices];
 
+// Whether the calling thread has a current context.
+bool has_context() {
+  using GetCurrent = CUresult (*)(CUcontext*);
+  static const GetCurrent get = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<GetCurrent>(p)
+               : nullptr;
+  }();
+  CUcontext c = nullptr;
+  return get && get(&c) == CUDA_SUCCESS && c != nullptr;
+}
+
 // Per-device set-up, once: address of the status word and the compute capability.
 int device_setup(int* dev_out, unsigned int** status) {
   int dev = 0;
@@ -43,10 +58,11 @@ int device_setup(int* dev_out, unsigned int** status) {
   if (!g_status_ptr[dev]) return TRIFAST_ERR_LAUNCH;
   if (g_arch_major[dev] != 10) return TRIFAST_ERR_ARCH;
   // A host thread that has not used the device yet (autograd's, if all memory came from a cache) has no
-  // current context, without which the driver refuses to encode a tensor map.
+  // current context, without which the driver refuses to encode a tensor map.  (A context that is there stays: a
+  // caller of the driver API may have one of its own, in which its memory and its stream lie.)
   static thread_local int bound = -1;
   if (bound != dev) {
-    if (cudaSetDevice(dev) != cudaSuccess) return TRIFAST_ERR_LAUNCH;
+    if (!has_context() && cudaSetDevice(dev) != cudaSuccess) return TRIFAST_ERR_LAUNCH;
     bound = dev;
   }
   *dev_out = dev;
