@@ -350,7 +350,8 @@ int trifast_backward_static_scratch(const trifast_shape* shape,
 
 /* Layer norm over the last dimension: y = (x - mean) / sqrt(var + eps) * weight + bias. */
 typedef struct trifast_norm {
-  int64_t rows;
+  int64_t rows;           /* at most 4,194,240 where a row, with what it shares its 16-byte pieces with, has more
+                             than 8192 elements */
   int64_t ld_x, ld_dy;    /* elements between rows of x and of dy: width plus a multiple of 16 bytes */
   int32_t width;          /* 1 .. 1048576 */
   int32_t dtype;          /* of x, y and their gradients */

@@ -36,3 +36,15 @@ def test_weight_sums_have_a_share_of_the_workspace_for_each_run():
         for rows in (128 * 128 * 40, 128 * 128 * 100):
             values = 3 * 2 * hidden * (-(-rows // 128) * 128)      # h, da, db of the chunk
             assert size(rows, width, hidden, 2) - values >= stride * (rows // (128 * 128))
+
+
+@pytest.mark.parametrize("width,dtype,rc", [(8192, 1, -1), (8188, 0, -1), (8192, 0, -1), (8185, 2, -1), (8184, 1, -1), (8186, 1, -12), (8190, 0, -12),
+                                            (8193, 0, -12), (8200, 2, -12)])
+def test_row_limit_of_layer_norm_is_that_of_long_rows(width, dtype, rc):
+    """Rows that a block holds in registers have none: the call goes on to its pointers."""
+    lib = _lib.load()
+    n = _lib.Norm(rows=4_194_241, ld_x=width, ld_dy=width, width=width, dtype=dtype, affine_dtype=0, eps=1e-5)
+    assert lib.trifast_layer_norm(C.byref(n), None, None, None, None, None) == rc
+    assert lib.trifast_layer_norm_backward(C.byref(n), *[None] * 7, 0, None) == rc
+    n.rows -= 1
+    assert lib.trifast_layer_norm(C.byref(n), None, None, None, None, None) == -1

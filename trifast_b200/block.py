@@ -69,7 +69,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x: (..., width), fp32, bf16 or fp16, with width at most 2**20; weight and bias: (width,), both of x's type or both fp32, or None
     (no affine part; a bias needs a weight).  Arithmetic is in fp32 and the result, of x's shape and type,
     is rounded once.  Differentiable, once, in x, weight and bias.  Rows may be strided; a tensor whose
-    leading dimensions cannot be walked with one stride is copied.
+    leading dimensions cannot be walked with one stride is copied.  Rows of more than 8192 elements (8185 where they are
+    not whole 16-byte pieces; fp32 8189): at most 4,194,240 of them.
     """
     return _layer_norm(x, weight, bias, eps)
 

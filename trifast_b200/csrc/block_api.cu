@@ -42,8 +42,9 @@ int check_norm(const trifast_norm* n, bool backward) {
   if (!(n->eps >= 0.f) || !isfinite(n->eps)) return TRIFAST_ERR_SHAPE;
   for (int64_t ld : {n->ld_x, backward ? n->ld_dy : n->ld_x})
     if (ld < n->width || (n->rows > 1 && !layer_norm_rows_fit(ld, n->width, n->dtype))) return TRIFAST_ERR_STRIDE;
-  // (rows longer than a block's registers are summed 64 to a block along the grid's second dimension)
-  if (n->width > 8192 - 7 && n->rows > (int64_t)65535 * 64) return TRIFAST_ERR_TOO_LARGE;
+  // (rows longer than a block's registers: their gradients' sums take 64 to a block along the grid's second dimension, and no
+  // forward pass is taken whose backward would not be)
+  if (layer_norm_in_passes(n->width, n->dtype) && n->rows > (int64_t)65535 * 64) return TRIFAST_ERR_TOO_LARGE;
   return TRIFAST_OK;
 }
 

@@ -16,6 +16,8 @@ struct LayerNormArgs {
 };
 // Whether rows `ld` elements apart begin at the same places of 16-byte pieces as dense ones: what the kernels take.
 bool layer_norm_rows_fit(int64_t ld, int width, int dtype);
+// Whether rows are too long for a block's registers.
+bool layer_norm_in_passes(int width, int dtype);
 // fp32 words of workspace that the gradients of weight and bias need.
 int64_t layer_norm_workspace_floats(int64_t rows, int width, int dtype);
 cudaError_t layer_norm_forward(const LayerNormArgs& a, cudaStream_t s);

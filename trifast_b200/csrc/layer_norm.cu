@@ -678,9 +678,11 @@ bool layer_norm_rows_fit(int64_t ld, int width, int dtype) {
   return (ld - width) % vec == 0;
 }
 
+bool layer_norm_in_passes(int width, int dtype) { return pieces_width(width, dtype == TRIFAST_F32 ? 4 : 8) > kMaxRow; }
+
 int64_t layer_norm_workspace_floats(int64_t rows, int width, int dtype) {
   const int vec = dtype == TRIFAST_F32 ? 4 : 8;
-  if (pieces_width(width, vec) > kMaxRow) return (rows + kLongRows - 1) / kLongRows * 2 * width + 2 * rows;
+  if (layer_norm_in_passes(width, dtype)) return (rows + kLongRows - 1) / kLongRows * 2 * width + 2 * rows;
   return bwd_blocks(rows, width, vec) * 2 * width;
 }
 
