@@ -371,7 +371,8 @@ int trifast_layer_norm_backward(const trifast_norm* norm, const void* dy, const 
 
 /* Gated feed-forward block: y = (silu(x w_gate^T) * (x w_up^T)) w_down^T, with w_gate and w_up
  * (hidden, width) and w_down (width_out, hidden), dense, all of one dtype.  Between the two
- * products the hidden values are held in that dtype. */
+ * products the hidden values are held in that dtype (forward passes of up to 8 rows: in fp32), and in the
+ * backward their gradients.  The fp16 ones beyond 65504 are infinite, below 2^-25 zero. */
 typedef struct trifast_ff {
   int64_t rows;
   int64_t ld_x, ld_dy;    /* elements between rows of x and of dy */

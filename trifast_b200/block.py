@@ -79,13 +79,14 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     """The gated feed-forward block ``(silu(x w_gate^T) * (x w_up^T)) w_down^T``.
 
     x: (..., width); w_gate, w_up: (hidden, width); w_down: (width_out, hidden), as a linear layer holds
-    them; all fp32, bf16 or fp16.  Returns (..., width_out) in x's type.  Sums are fp32; the hidden
+    them; all fp32, bf16 or fp16, at most 65536 wide.  Returns (..., width_out) in x's type.  Sums are fp32; the hidden
     values are rounded to x's type between the two products (fp16: a hidden value beyond 65504 is infinite),
-    and so are their gradients in the backward, which computes the hidden values again instead of keeping
-    them: nothing but the arguments is saved, and the workspace of a call does not grow with the number of
-    rows.  fp32 products are as exact as fp32 sums, but a row with an infinite value in x or a weight gives
-    NaN there.  The forward pass of up to eight rows runs on the CUDA cores with fp32 hidden values: its last
-    bits may differ from those of the same rows in a larger batch.  Differentiable, once, in all four.
+    and so are their gradients in the backward (fp16: those below 2**-25 are 0), which computes the hidden values
+    again instead of keeping them: nothing but the arguments is saved, and the workspace of a call does not
+    grow with the number of rows beyond a chunk of them.  fp32 products are as exact as fp32 sums, but an infinite
+    value in x, a weight or between the products gives NaN there.  The forward pass of up to eight rows runs on the
+    CUDA cores with fp32 hidden values: its last bits may differ from those of the same rows in a larger batch, where
+    an fp16 hidden value beyond 65504 is infinite.  Differentiable, once, in all four.
     """
     return _gated_feed_forward(x, w_gate, w_up, w_down)
 

@@ -75,8 +75,9 @@ int check_ff(const trifast_ff* f, bool backward) {
 
 int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
-// Rows are worked on in chunks, whose hidden values (and, backward, their gradients) lie in the workspace, of at most
-// this many bytes whatever the number of rows.  (48 MB, which stay in L2 from one kernel to the next, lost more to the
+// Rows are worked on in chunks, whose hidden values (and, backward, their gradients) and operands laid out anew lie in the
+// workspace, of at most this many bytes whatever the number of rows, but of 1024 rows at least (hidden 65536, backward: 403 MB in
+// 16 bits, 1.2 GB in fp32).  (48 MB, which stay in L2 from one kernel to the next, lost more to the
 // last rounds of tiles than they saved: 65,536 rows, width 512, hidden 1024 forward 198 us in three chunks.)
 constexpr int64_t kChunkBytes = 256 << 20;
 

@@ -15,9 +15,11 @@
 // kernel adds up.  S is computed three times in all (forward, dX, dW) and dH twice, five products of fourteen, against six
 // hidden-sized tensors through memory.
 //
-// 1,048,576 rows, width 128, hidden 512, bf16: forward 334 us, dX 545, dW 742, 1.23, 1.26 and 1.11 PFLOP/s of what they
-// run.  Forward and dX are near what the chip sustains (cuBLAS: 1.36); what bounds dW is shared memory: 336 KB of operands
-// read, rows fetched and gradients staged per 128 rows, 2,625 of 2,900 cycles at 128 bytes a cycle.
+// 1,048,576 rows, width 128, hidden 512, bf16: forward 335 us, dX 549, dW 767, 1.23, 1.25 and 1.08 PFLOP/s of what they
+// run, on a chip that was idle before; under load 389, 639 and 862.  Forward and dX are near what the chip sustains (cuBLAS: 1.36).
+// dW: operands, rows fetched and gradients staged are 336 KB of shared memory per 128 rows, which at 128 bytes a cycle would be
+// 2,625 of its 2,900 cycles.  The counters show no unit at its limit: reads of operands 55 % of the wavefronts, tensor pipe
+// 47 %.
 //
 // All waits are bounded.
 

@@ -18,11 +18,11 @@
 //
 // fp32: every value is the sum of three bf16 ones (ff_support.cu), and a product is the six products of parts that are not
 // below 2^-22 of it.  A stage holds all three parts of both operands.  The accumulators in TMEM round towards zero, so
-// that a long sum drifts (5e-6 of the result over 384 MMAs): a sum takes one stage, the smallest products first, and
+// that a long sum drifts (1.0e-7 of a sum of positive terms with every MMA): a sum takes one stage, the smallest products first, and
 // the epilogue adds the sums up in fp32 registers, rounded to nearest.
 //
 // What bounds it: the tiles' way from L2.  A pair's 256 x 256 tile takes 32 KB a CTA per 64 of the contraction, which the
-// tensor pipe works on for 512 cycles: 64 bytes a cycle, of which about 42 arrive (10.7 TB/s on all SMs).  65,536 rows of
+// tensor pipe works on for 512 cycles: 64 bytes a cycle, of which about 41 arrive (9.4 TB/s on all SMs).  65,536 rows of
 // 512, hidden 1024, bf16: 110 us for the gate, 56 for the result, 1.25 PFLOP/s.
 
 #include <initializer_list>

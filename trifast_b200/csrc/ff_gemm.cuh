@@ -62,7 +62,8 @@ struct FewArgs {
 cudaError_t few_rows(const FewArgs& a, cudaStream_t s);
 bool few_rows_in_cluster(int64_t rows, int64_t width, int64_t hidden, int64_t width_out, int elem);   // (needs no h)
 
-// dst (dst.planes planes, rows padded with zeros to dst.rows) from src (rows x dst.cols of the call's type, `ld` apart).
+// dst (dst.planes planes, columns padded with zeros to dst.pitch) from src (rows x dst.cols of the call's type, `ld` apart).
+// Rows behind the last are left as they are: the tensor maps end before them.
 struct StageJob {
   const void* src;
   int64_t ld, rows;
