@@ -72,5 +72,5 @@ def keep_mask(shape, p, seed, offset=0, shared_dim=None):
 
 
 def dropout_add(x, residual, keep, p):
-    y = torch.where(keep, x.double() / (1 - p) if p < 1 else 0.0, 0.0)
+    y = torch.where(keep, x.double() / (1 - p) if p < 1 else 0.0, 0.0).expand(x.shape)
     return y if residual is None else y + residual.double()
